@@ -196,6 +196,44 @@ int tn_adam_step_plan(tn_plan* p, float* params, const float* grads, float* exp_
  * OUTSIDE the captured graph, before each replay). */
 int tn_plan_set_lr(tn_plan* p, float lr, void* stream);
 
+/* ---- AdamW over many tensors at once (new; the reference steps one torch.optim.Adam, src/train.py:131-135) ------------------
+ * m' = b1 m + (1 - b1) g, v' = b2 v + (1 - b2) g^2 (g times the clipping factor),
+ * p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps).
+ * The moments of all tensors lie in one buffer in blocks of TN_OPT_BLOCK = 256 elements; tensor i has its own from first_block[i]
+ * on (the rest of its last block is padding and holds zeros).  state_bits 32: float moments.  state_bits 8: one byte per element and one float scale
+ * per block,  exp_avg = sign (c / 127)^2 scale,  exp_avg_sq = (c / 255)^4 scale, nearest code, the lower one half way, and no
+ * exp_avg_sq above 0 gets code 0; a block with a NaN or an infinity gets the scale NaN.
+ * A step is: tn_grad_sumsq for each list of gradients and tn_grad_norm_finish (where the norm clips), tn_adamw_tick once for
+ * each set of hyper-parameters, tn_adamw_apply for each list of tensors of one type.  Everything that changes from step to step
+ * (counts, factor, learning rate) is in device memory: the sequence can be captured.
+ * Pointer arrays are HOST arrays and are not read after the call returns.  numel may be 0. */
+#define TN_OPT_BLOCK 256
+#define TN_DTYPE_F32 0
+#define TN_DTYPE_BF16 1
+#define TN_DTYPE_F16 2
+/* how many partial sums tn_grad_sumsq writes at most for these tensors */
+int64_t tn_grad_sumsq_partials(int32_t count, const int64_t* numel);
+/* partials: device double; *written (host): how many of them hold a sum */
+int tn_grad_sumsq(int32_t count, const void* const* grads, const int64_t* numel, int32_t dtype, double* partials, int64_t* written,
+                  void* stream);
+/* norm (device float, may be NULL) = |grad_mult| sqrt(sum of the partials).  ctl (device double[2], may be NULL): {grad_mult *
+ * min(1, max_norm / (norm + 1e-6)), 1}, or {0, 0} where the norm is not finite: the step that reads it changes nothing then. */
+int tn_grad_norm_finish(const double* partials, int64_t count, double grad_mult, double max_norm, float* norm, double* ctl, void* stream);
+/* steps (device int32), corr (device float[4] each) are indexed by slot: tensors that have always been stepped together share
+ * one.  Advances the count of each listed slot and derives its bias corrections.  lr_dev (device float) replaces lr if given. */
+int tn_adamw_tick(int32_t count, const int32_t* slots, int32_t* steps, float* corr, const double* ctl, double lr, const float* lr_dev,
+                  double beta1, double beta2, double weight_decay, void* stream);
+/* blocks: how many the moment buffers hold.  ctl NULL: gradients times grad_mult. */
+int tn_adamw_apply(int32_t count, void* const* params, const void* const* grads, const int64_t* numel, const int64_t* first_block,
+                   const int32_t* slots, int32_t dtype, int32_t state_bits, void* exp_avg, void* exp_avg_sq, float* scale1, float* scale2,
+                   int64_t blocks, const float* corr, const double* ctl, double grad_mult, double beta1, double beta2, double eps,
+                   void* stream);
+/* 8-bit moments -> float values [blocks * 256] and back */
+int tn_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale1, const float* scale2, float* out1, float* out2,
+                      int64_t blocks, void* stream);
+int tn_moments_encode(const float* in1, const float* in2, void* exp_avg, void* exp_avg_sq, float* scale1, float* scale2, int64_t blocks,
+                      void* stream);
+
 /* ---- stand-alone loss heads: MetricLearningLoss.forward(inputs, targets) -> (normalised inputs, preds, loss)
  * (reference src/losses.py:32-44 CELoss, :77-132 AngularMarginLoss) for callers that use a loss object outside
  * TitaNet.forward.  loss_type: TN_LOSS_CE (fc_bias required) or TN_LOSS_MARGIN (fc_weight is row-normalised IN PLACE, as

@@ -1,0 +1,87 @@
+"""Refusals of the optimizer step and the gradient norm, and the oracle's 8-bit moments: no GPU needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from tests import optim_oracle as O
+from titanet_amd import _lib
+from titanet_amd.optim import AdamW, grad_norm
+
+
+def test_parameters_must_live_on_a_device():
+    with pytest.raises(RuntimeError, match="no CPU execution path"):
+        AdamW([torch.zeros(4)])
+    with pytest.raises(RuntimeError, match="no CPU execution path"):
+        grad_norm([torch.zeros(4)])
+
+
+@pytest.mark.parametrize("kw", [dict(lr=-1.0), dict(lr=float("nan")), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+                                dict(state_bits=16), dict(max_grad_norm=0.0), dict(max_grad_norm=float("nan")), dict(lr=torch.zeros(2)),
+                                dict(lr=torch.zeros((), dtype=torch.float64))])
+def test_hyper_parameters_out_of_range(kw):
+    with pytest.raises(ValueError):
+        AdamW([torch.zeros(4)], **kw)
+
+
+@pytest.mark.parametrize("p", [torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int64), torch.zeros(4).to_sparse()])
+def test_types_it_does_not_take(p):
+    with pytest.raises(TypeError):
+        AdamW([p])
+    with pytest.raises(TypeError):
+        grad_norm([p])
+    with pytest.raises(TypeError):
+        AdamW([1.0])
+
+
+def test_grad_norm_of_nothing():
+    with pytest.raises(ValueError):
+        grad_norm([])
+
+
+def test_c_entries_refuse_before_they_touch_the_device():
+    lib = _lib.load()
+    one, none = (C.c_void_p * 1)(4096), C.c_void_p(0)
+    n, first, slot = (C.c_int64 * 1)(256), (C.c_int64 * 1)(0), (C.c_int32 * 1)(0)
+    at, written = C.c_void_p(4096), C.c_int64()
+
+    def apply(count=1, params=one, numel=n, first_block=first, slots=slot, dtype=0, bits=32, m=at, scale=at, blocks=1, b1=0.9, eps=1e-8):
+        return lib.tn_adamw_apply(count, params, one, numel, first_block, slots, dtype, bits, m, at, scale, scale, blocks, at, none, 1.0, b1, 0.999,
+                                  eps, none)
+
+    bad, unsupported = -1, -2
+    assert apply(count=0) == 0 and apply(count=-1) == bad
+    assert apply(params=(C.c_void_p * 1)(0)) == bad and apply(m=none) == bad
+    assert apply(numel=(C.c_int64 * 1)(-1)) == bad and apply(slots=(C.c_int32 * 1)(-1)) == bad
+    assert apply(numel=(C.c_int64 * 1)(257)) == bad                      # more than the moment buffers hold
+    assert apply(first_block=(C.c_int64 * 1)(1)) == bad and apply(first_block=(C.c_int64 * 1)(-1)) == bad
+    assert apply(dtype=3) == unsupported and apply(bits=16) == unsupported and apply(bits=8, scale=none) == bad
+    assert apply(b1=1.0) == bad and apply(b1=float("nan")) == bad and apply(eps=-1.0) == bad and apply(blocks=1 << 33) == unsupported
+    assert lib.tn_grad_sumsq_partials(-1, none) == bad and lib.tn_grad_sumsq_partials(0, none) == 0
+    assert lib.tn_grad_sumsq_partials(1, n) == 1 and lib.tn_grad_sumsq_partials(1, (C.c_int64 * 1)(16385)) == 2
+    assert lib.tn_grad_sumsq(1, one, n, 7, at, C.byref(written), none) == unsupported
+    assert lib.tn_grad_sumsq(1, (C.c_void_p * 1)(0), n, 0, at, C.byref(written), none) == bad
+    assert lib.tn_grad_norm_finish(at, -1, 1.0, 1.0, at, none, none) == bad and lib.tn_grad_norm_finish(at, 1, 1.0, 0.0, at, at, none) == bad
+    assert lib.tn_adamw_tick(1, slot, at, none, none, 1e-3, none, 0.9, 0.999, 0.0, none) == bad
+    assert lib.tn_adamw_tick(1, slot, at, at, none, -1.0, none, 0.9, 0.999, 0.0, none) == bad
+    assert lib.tn_adamw_tick(1, (C.c_int32 * 1)(-1), at, at, none, 1e-3, none, 0.9, 0.999, 0.0, none) == bad
+    assert lib.tn_moments_decode(none, at, at, at, at, at, 1, none) == bad and lib.tn_moments_encode(at, at, at, at, at, none, 1, none) == bad
+
+
+def test_oracle_codes_are_the_nearest_and_survive_a_round_trip():
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal(700) * np.exp(rng.standard_normal(700))
+    for second in (False, True):
+        y = x * x if second else x
+        code, top = O.encode(y, second)
+        back = O.decode(code, top, second)
+        again, top2 = O.encode(back, second)
+        assert np.array_equal(code, again) and np.array_equal(top, top2)
+        # in the root's domain the codes are even steps: no value is further than half a step away (code 1 takes all below it)
+        root = (lambda a: np.abs(a) ** 0.25) if second else (lambda a: np.abs(a) ** 0.5)
+        scale = np.repeat(root(top.astype(np.float64)), O.BLOCK)[:700]
+        off = np.abs(root(y) - root(back)) / scale
+        step = 1 / 255 if second else 1 / 127
+        assert off[code != 1].max() <= step / 2 * (1 + 1e-6) and off.max() <= step
+        assert not second or (code[y > 0] >= 1).all()

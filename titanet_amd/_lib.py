@@ -19,7 +19,8 @@ EXPORTS = [
     "tn_profile_read", "tn_profile_sample", "tn_mel_create", "tn_mel_destroy", "tn_mel_num_frames", "tn_mel_forward", "tn_mel_forward_batch", "tn_plan_step_tick",
     "tn_plan_step_set", "tn_adam_step_plan", "tn_plan_set_lr", "tn_head_save_floats", "tn_head_forward", "tn_head_backward",
     "tn_forward_masked", "tn_forward_prepacked", "tn_plan_prolog_input", "tn_mel_forward_batch_packed", "tn_plan_set_grad_groups", "tn_plan_num_grad_buckets", "tn_plan_grad_bucket", "tn_plan_wait_grad_bucket",
-    "tn_mark_host",
+    "tn_mark_host", "tn_grad_sumsq_partials", "tn_grad_sumsq", "tn_grad_norm_finish", "tn_adamw_tick", "tn_adamw_apply", "tn_moments_decode",
+    "tn_moments_encode",
 ]
 
 
@@ -104,6 +105,15 @@ def load():
     lib.tn_plan_prolog_input.argtypes = [vp]
     lib.tn_plan_prolog_input.restype = vp
     lib.tn_forward_prepacked.argtypes = [vp, vp, vp, i32, C.c_uint64, vp, vp, vp, vp]
+    f64 = C.c_double
+    lib.tn_grad_sumsq_partials.argtypes = [i32, vp]
+    lib.tn_grad_sumsq_partials.restype = i64
+    lib.tn_grad_sumsq.argtypes = [i32, vp, vp, i32, vp, C.POINTER(i64), vp]
+    lib.tn_grad_norm_finish.argtypes = [vp, i64, f64, f64, vp, vp, vp]
+    lib.tn_adamw_tick.argtypes = [i32, vp, vp, vp, vp, f64, vp, f64, f64, f64, vp]
+    lib.tn_adamw_apply.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64, vp, vp, f64, f64, f64, f64, vp]
+    lib.tn_moments_decode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.tn_moments_encode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
     lib.tn_version.restype = C.c_char_p
     for name in EXPORTS:
         fn = getattr(lib, name)
