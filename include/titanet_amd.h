@@ -234,6 +234,19 @@ int tn_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* 
 int tn_moments_encode(const float* in1, const float* in2, void* exp_avg, void* exp_avg_sq, float* scale1, float* scale2, int64_t blocks,
                       void* stream);
 
+/* ---- matrix product in 8-bit integers with a scale for each token and each channel (new; the reference multiplies in float32,
+ * nn.Linear of src/losses.py:30 and the cosine scores of src/learn.py:441-447) --------------------------------------------------
+ *   y[m][n] = a_scales[m] b_scales[n] sum_k a[m][k] b[n][k] (+ bias[n])           the sum in 32-bit integers, exact
+ * Codes are int8 [rows][ld], ld a multiple of 64, base 16-byte aligned, zeros from k to the next multiple of 64.
+ * tn_int8_quantize_rows makes them from float rows of any stride: scale = max(max |row| / 127, 2^-126) (0 for a row of zeros), code
+ * = x / scale rounded to the nearest integer, even half way; a row with a NaN or an infinity gets the scale NaN and codes 0 (its
+ * products are NaN). */
+#define TN_INT8_MAX_K 131071
+int tn_int8_quantize_rows(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx, void* codes, int64_t ld_codes,
+                          float* scales, void* stream);
+int tn_int8_matmul(const void* a, const float* a_scales, int64_t lda, const void* b, const float* b_scales, int64_t ldb, const float* bias,
+                   void* y, int32_t y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, void* stream);
+
 /* ---- stand-alone loss heads: MetricLearningLoss.forward(inputs, targets) -> (normalised inputs, preds, loss)
  * (reference src/losses.py:32-44 CELoss, :77-132 AngularMarginLoss) for callers that use a loss object outside
  * TitaNet.forward.  loss_type: TN_LOSS_CE (fc_bias required) or TN_LOSS_MARGIN (fc_weight is row-normalised IN PLACE, as

@@ -1,0 +1,53 @@
+"""Refusals of the 8-bit product: no GPU needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+from titanet_amd import _lib
+from titanet_amd.int8 import Int8Linear, Int8Rows, int8_matmul, quantize_rows
+
+
+def test_operands_must_live_on_a_device():
+    for call in (lambda: quantize_rows(torch.ones(2, 3)), lambda: Int8Rows(torch.ones(2, 3, dtype=torch.int8), torch.ones(2)),
+                 lambda: Int8Linear(torch.ones(2, 3))):
+        with pytest.raises(RuntimeError, match="no CPU execution path"):
+            call()
+
+
+def test_types_and_shapes_it_does_not_take():
+    for bad in (torch.ones(2, 3, dtype=torch.float64), torch.ones(2, 3, dtype=torch.int8), [1.0]):
+        with pytest.raises(TypeError):
+            quantize_rows(bad)
+    for bad in (torch.ones(3), torch.ones(2, 3, 4), torch.ones(2, 0), torch.empty(1, 131072)):
+        with pytest.raises(ValueError):
+            quantize_rows(bad)
+    with pytest.raises(TypeError):
+        Int8Rows(torch.ones(2, 3), torch.ones(2))
+    with pytest.raises(TypeError):
+        Int8Rows(torch.ones(2, 3, dtype=torch.int8), torch.ones(3))
+    with pytest.raises(TypeError):
+        Int8Rows(torch.ones(2, 3, dtype=torch.int8), torch.ones(2, dtype=torch.float64))
+    with pytest.raises(TypeError):
+        int8_matmul(torch.ones(2, 3), torch.ones(2, 3))
+
+
+def test_c_entries_refuse_before_they_touch_the_device():
+    lib = _lib.load()
+    at, none = C.c_void_p(4096), C.c_void_p(0)
+    bad, unsupported = -1, -2
+
+    def quantize(x=at, dtype=0, rows=1, cols=3, ldx=3, ld=64, scales=at):
+        return lib.tn_int8_quantize_rows(x, dtype, rows, cols, ldx, at, ld, scales, none)
+
+    assert quantize(rows=0) == 0 and quantize(rows=-1) == bad and quantize(x=none) == bad and quantize(scales=none) == bad
+    assert quantize(cols=0) == bad and quantize(ld=63) == bad and quantize(cols=65) == bad and quantize(ldx=-1) == bad
+    assert quantize(dtype=3) == unsupported and quantize(cols=131072, ld=131072) == unsupported
+
+    def matmul(a=at, b=at, y=at, dtype=0, lda=64, ldb=64, ldy=5, m=4, n=5, k=3):
+        return lib.tn_int8_matmul(a, at, lda, b, at, ldb, none, y, dtype, ldy, m, n, k, none)
+
+    assert matmul(m=0) == 0 and matmul(n=0) == 0 and matmul(m=-1) == bad and matmul(k=0) == bad
+    assert matmul(a=none) == bad and matmul(y=none) == bad and matmul(b=C.c_void_p(4097)) == bad
+    assert matmul(lda=32) == bad and matmul(k=65) == bad and matmul(ldy=4) == bad
+    assert matmul(dtype=-1) == unsupported and matmul(lda=131072, ldb=131072, k=131072) == unsupported

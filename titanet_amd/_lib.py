@@ -20,7 +20,7 @@ EXPORTS = [
     "tn_plan_step_set", "tn_adam_step_plan", "tn_plan_set_lr", "tn_head_save_floats", "tn_head_forward", "tn_head_backward",
     "tn_forward_masked", "tn_forward_prepacked", "tn_plan_prolog_input", "tn_mel_forward_batch_packed", "tn_plan_set_grad_groups", "tn_plan_num_grad_buckets", "tn_plan_grad_bucket", "tn_plan_wait_grad_bucket",
     "tn_mark_host", "tn_grad_sumsq_partials", "tn_grad_sumsq", "tn_grad_norm_finish", "tn_adamw_tick", "tn_adamw_apply", "tn_moments_decode",
-    "tn_moments_encode",
+    "tn_moments_encode", "tn_int8_quantize_rows", "tn_int8_matmul",
 ]
 
 
@@ -114,6 +114,8 @@ def load():
     lib.tn_adamw_apply.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64, vp, vp, f64, f64, f64, f64, vp]
     lib.tn_moments_decode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
     lib.tn_moments_encode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.tn_int8_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]
+    lib.tn_int8_matmul.argtypes = [vp, vp, i64, vp, vp, i64, vp, vp, i32, i64, i64, i64, i64, vp]
     lib.tn_version.restype = C.c_char_p
     for name in EXPORTS:
         fn = getattr(lib, name)

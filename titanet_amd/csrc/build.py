@@ -14,7 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
-SOURCES = ["tn_api.hip", "tn_bwd.hip", "tn_mel.hip", "tn_optim.hip"]
+SOURCES = ["tn_api.hip", "tn_bwd.hip", "tn_mel.hip", "tn_optim.hip", "tn_int8.hip"]
 # every header next to the sources feeds the rebuild digest (a stale .so must never ship: it travels prebuilt)
 HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".h")) + ["../../include/titanet_amd.h"]
 OUT = os.path.join(PKG, "libtitanet_amd.so")

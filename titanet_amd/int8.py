@@ -1,0 +1,162 @@
+"""Matrix products in 8-bit integers with a scale for each token and each channel.
+
+    gallery = quantize_rows(enrolled)                       # [speakers, E] float -> codes and scales, once
+    scores = int8_matmul(embeddings, gallery)               # [utterances, speakers]: the embeddings are quantised in the call
+    head = Int8Linear.from_linear(loss.fc)                  # a head or any other linear layer, for serving
+
+The reference multiplies in float32 (the heads' ``nn.Linear``, reference src/losses.py:30; the cosine scores of its test, reference
+src/learn.py:441-447).  Here both operands are int8 rows with one float32 scale each, the sums are exact 32-bit integers
+(``tn_int8_matmul``, include/titanet_amd.h) and one multiplication by both scales follows.  For serving: there is no backward
+pass and no CPU fallback.
+"""
+import ctypes as C
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import check
+
+MAX_K = 131071       # TN_INT8_MAX_K: 128 * 128 * MAX_K still fits 32 bits
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _p(t):
+    return C.c_void_p(t.data_ptr() if t is not None else 0)
+
+
+def _need_device(t, what):
+    if not t.is_cuda:
+        raise RuntimeError(f"titanet_amd.int8: {what} must be a ROCm device tensor; there is no CPU execution path")
+
+
+class Int8Rows:
+    """Rows of int8 codes with a float32 scale each: row r stands for ``scales[r] * codes[r]``.  Held with every row padded by
+    zeros to a multiple of 64 bytes, as the product reads them; ``codes`` is the unpadded view."""
+
+    def __init__(self, codes, scales):
+        if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] < 1:
+            raise TypeError(f"codes must be an int8 matrix, got {codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],):
+            raise TypeError(f"scales must be float32, one for each of the {codes.shape[0]} rows, got {scales.dtype} {tuple(scales.shape)}")
+        if codes.shape[1] > MAX_K:
+            raise ValueError(f"rows of more than {MAX_K} codes could overflow the 32-bit sums")
+        _need_device(codes, "codes")
+        if scales.device != codes.device:
+            raise ValueError(f"codes and scales are on different devices: {codes.device} and {scales.device}")
+        rows, cols = codes.shape
+        padded = torch.zeros(rows, (cols + 63) // 64 * 64, dtype=torch.int8, device=codes.device)
+        padded[:, :cols] = codes.detach()
+        self._padded, self.scales, self.cols = padded, scales.detach().contiguous(), cols
+
+    @classmethod
+    def _of(cls, padded, scales, cols):
+        r = cls.__new__(cls)
+        r._padded, r.scales, r.cols = padded, scales, cols
+        return r
+
+    @property
+    def codes(self):
+        return self._padded[:, :self.cols]
+
+    @property
+    def shape(self):
+        return torch.Size((self._padded.shape[0], self.cols))
+
+    @property
+    def device(self):
+        return self._padded.device
+
+    def __len__(self):
+        return self._padded.shape[0]
+
+    def dequantize(self):
+        """the float32 values the rows stand for"""
+        return self.codes.float() * self.scales[:, None]
+
+
+def quantize_rows(x):
+    """``Int8Rows`` of a float matrix (float32, bfloat16 or float16): scale max |row| / 127 (at least 2^-126; 0 for a row of
+    zeros), codes the nearest integers to x / scale, even half way.  A row with a NaN or an infinity gets the scale NaN."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
+        raise TypeError(f"quantize_rows takes a float32, bfloat16 or float16 matrix, got {getattr(x, 'dtype', type(x))}")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"quantize_rows takes a matrix with at least one column, got {tuple(x.shape)}")
+    if x.shape[1] > MAX_K:
+        raise ValueError(f"rows of more than {MAX_K} values could overflow the 32-bit sums")
+    _need_device(x, "x")
+    x = x.detach()
+    if x.stride(1) != 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    rows, cols = x.shape
+    with torch.cuda.device(x.device):
+        padded = torch.empty(rows, (cols + 63) // 64 * 64, dtype=torch.int8, device=x.device)
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        check(_lib.load().tn_int8_quantize_rows(_p(x), _TYPES[x.dtype], rows, cols, x.stride(0), _p(padded), padded.shape[1], _p(scales),
+                                                C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)), "tn_int8_quantize_rows")
+    return Int8Rows._of(padded, scales, cols)
+
+
+def int8_matmul(a, b, bias=None, out_dtype=None):
+    """``a @ b.T (+ bias)`` in 8-bit integers: ``b`` an :class:`Int8Rows` [N, K], ``a`` one of [M, K] or a float tensor [..., K]
+    whose rows are quantised in the call; ``bias`` float32 [N].  Returns [..., N] in ``out_dtype`` (float32, bfloat16, float16;
+    default: that of a float ``a``, else float32)."""
+    if not isinstance(b, Int8Rows):
+        raise TypeError(f"the second operand must be Int8Rows (quantize_rows), got {type(b).__name__}")
+    if isinstance(a, torch.Tensor):
+        if a.dtype not in _TYPES:
+            raise TypeError(f"the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got {a.dtype}")
+        if a.dim() < 1:
+            raise ValueError("the first operand needs at least one dimension")
+        if torch.is_grad_enabled() and (a.requires_grad or (bias is not None and bias.requires_grad)):
+            raise RuntimeError("int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()")
+        lead, cols, dtype = a.shape[:-1], a.shape[-1], a.dtype
+    elif isinstance(a, Int8Rows):
+        lead, cols, dtype = (len(a),), a.cols, torch.float32
+    else:
+        raise TypeError(f"the first operand must be Int8Rows or a tensor, got {type(a).__name__}")
+    out_dtype = dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if cols != b.cols:
+        raise ValueError(f"operands of {cols} and {b.cols} columns")
+    if a.device != b.device:
+        raise ValueError(f"operands on different devices: {a.device} and {b.device}")
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (len(b),) or bias.device != b.device:
+            raise ValueError(f"bias must be float32 [{len(b)}] on {b.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+        bias = bias.detach().contiguous()
+    if isinstance(a, torch.Tensor):
+        a = quantize_rows(a.detach().reshape(-1, cols))
+    m, n = len(a), len(b)
+    with torch.cuda.device(b.device):
+        y = torch.empty(m, n, dtype=out_dtype, device=b.device)
+        check(_lib.load().tn_int8_matmul(_p(a._padded), _p(a.scales), a._padded.shape[1], _p(b._padded), _p(b.scales), b._padded.shape[1],
+                                         _p(bias), _p(y), _TYPES[out_dtype], n, m, n, cols,
+                                         C.c_void_p(torch.cuda.current_stream(b.device).cuda_stream)), "tn_int8_matmul")
+    return y.view(*lead, n)
+
+
+class Int8Linear(nn.Module):
+    """A linear layer for serving: int8 weight rows with a scale per output channel, inputs quantised per token in the call."""
+
+    def __init__(self, weight, bias=None):
+        super().__init__()
+        rows = quantize_rows(weight)
+        self.in_features, self.out_features = rows.cols, len(rows)
+        self.register_buffer("codes", rows._padded)
+        self.register_buffer("scales", rows.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
+
+    @classmethod
+    def from_linear(cls, module):
+        """from a module with ``weight`` [out, in] and optionally ``bias`` (an ``nn.Linear``, a loss head's ``fc``)"""
+        return cls(module.weight, getattr(module, "bias", None))
+
+    def forward(self, x, out_dtype=None):
+        if self.scales.dtype != torch.float32:
+            raise TypeError("Int8Linear keeps float32 scales: do not convert it to another type")
+        return int8_matmul(x, Int8Rows._of(self.codes, self.scales, self.in_features), bias=self.bias, out_dtype=out_dtype)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
