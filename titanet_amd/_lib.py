@@ -39,7 +39,7 @@ class TitaNetLibraryError(RuntimeError):
     pass
 
 
-_lib = None
+_lib = _host = None
 
 
 def load():
@@ -123,6 +123,21 @@ def load():
             fn.restype = C.c_int
     _lib = lib
     return lib
+
+
+def load_host():
+    """The Python module over torch tensors that stands next to the library (built by the same script)."""
+    global _host
+    if _host is None:
+        load()
+        import torch  # noqa: F401  (its libraries come first)
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise TitaNetLibraryError("titanet_amd/_host.so is missing or does not fit this torch: build it with "
+                                      f"`python titanet_amd/csrc/build.py` ({e})") from e
+        _host = module
+    return _host
 
 
 def check(rc, what):

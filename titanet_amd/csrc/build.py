@@ -18,6 +18,7 @@ SOURCES = ["tn_api.hip", "tn_bwd.hip", "tn_mel.hip", "tn_optim.hip", "tn_int8.hi
 # every header next to the sources feeds the rebuild digest (a stale .so must never ship: it travels prebuilt)
 HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".h")) + ["../../include/titanet_amd.h"]
 OUT = os.path.join(PKG, "libtitanet_amd.so")
+HOST_SOURCE, HOST_OUT = "tn_host.cpp", os.path.join(PKG, "_host.so")      # Python module over torch tensors, linked to the library
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
          "-Wno-unused-variable"]
 
@@ -29,7 +30,7 @@ NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 def _digest():
     h = hashlib.sha256()
-    for f in SOURCES + HEADERS + ["build.py"]:
+    for f in SOURCES + HEADERS + [HOST_SOURCE, "build.py"]:
         path = os.path.join(HERE, f)
         if os.path.exists(path):
             with open(path, "rb") as fh:
@@ -37,11 +38,26 @@ def _digest():
     return h.hexdigest()
 
 
+def _build_host(verbose):
+    import sysconfig
+
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-I" + os.path.join(base, "include"), "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), "-I" + sysconfig.get_paths()["include"],
+           os.path.join(HERE, HOST_SOURCE), "-o", HOST_OUT, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+           "-ltorch_python", "-L" + PKG, "-l:" + os.path.basename(OUT), "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+
+
 def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     stamp = os.path.join(HERE, ".build_stamp")
     dig = _digest()
-    if not force and os.path.exists(OUT) and os.path.exists(stamp) and open(stamp).read().strip() == dig:
+    if not force and os.path.exists(OUT) and os.path.exists(HOST_OUT) and os.path.exists(stamp) and open(stamp).read().strip() == dig:
         return OUT
     objs = []
 
@@ -59,6 +75,7 @@ def build(force=False, verbose=True):
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+    _build_host(verbose)
     with open(stamp, "w") as fh:
         fh.write(dig)
     return OUT

@@ -1,0 +1,353 @@
+// titanet_amd — host side of the optimizer step and of the 8-bit product for torch tensors (Python module titanet_amd._host).
+//
+// The kernels of these operators take microseconds; reading a few hundred tensors' addresses, types and gradients through Python
+// took longer than the step of a whole model (560 us against 48 us of kernels for 428 tensors).  What is checked and collected in
+// every call is therefore done here, and the launches go through the C entries of libtitanet_amd.so like every other caller's.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <array>
+#include <cmath>
+#include <optional>
+#include <vector>
+
+#include "../../include/titanet_amd.h"
+
+namespace py = pybind11;
+
+namespace {
+
+int type_code(c10::ScalarType t) {
+  return t == at::kFloat ? TN_DTYPE_F32 : t == at::kBFloat16 ? TN_DTYPE_BF16 : t == at::kHalf ? TN_DTYPE_F16 : -1;
+}
+
+void check(int rc, const char* what) {
+  TORCH_CHECK(rc == 0, what, " failed: ", rc == TN_E_BADARG ? "TN_E_BADARG" : rc == TN_E_UNSUPPORTED ? "TN_E_UNSUPPORTED" : "hipError_t ", rc > 0 ? std::to_string(rc) : "");
+}
+
+void* current_stream(const c10::Device& d) { return (void*)c10::hip::getCurrentHIPStream(d.index()).stream(); }
+
+// ------------------------------------------------------------------------------------------------------------- optimizer
+struct Lists {                         // the tensors of one type that a step touches
+  std::vector<void*> p;
+  std::vector<const void*> g;
+  std::vector<int64_t> numel, first;
+  std::vector<int32_t> index, slot;
+};
+
+struct GroupWork {
+  std::array<Lists, 3> by_type;
+  std::vector<int32_t> slots;
+  double lr, b1, b2, eps, wd;
+  at::Tensor lr_dev;
+};
+
+struct Norm {                          // partial sums of several lists, then their norm
+  static int64_t partials(const std::vector<std::pair<int, Lists*>>& lists) {
+    int64_t n = 0;
+    for (auto& [code, l] : lists) n += tn_grad_sumsq_partials((int32_t)l->numel.size(), l->numel.data());
+    return n;
+  }
+  static int64_t sums(const std::vector<std::pair<int, Lists*>>& lists, double* out, void* stream) {
+    int64_t at = 0, written = 0;
+    for (auto& [code, l] : lists) {
+      check(tn_grad_sumsq((int32_t)l->numel.size(), l->g.data(), l->numel.data(), code, out + at, &written, stream), "tn_grad_sumsq");
+      at += written;
+    }
+    return at;
+  }
+};
+
+class Stepper {
+ public:
+  Stepper(int bits) : bits_(bits) {}
+
+  void layout(std::vector<int64_t> numel, std::vector<int64_t> first, std::vector<int32_t> slots, int64_t blocks, at::Tensor exp_avg,
+              at::Tensor exp_avg_sq, std::optional<at::Tensor> scale1, std::optional<at::Tensor> scale2, at::Tensor steps, at::Tensor corr) {
+    numel_ = std::move(numel);
+    first_ = std::move(first);
+    blocks_ = blocks;
+    exp_avg_ = exp_avg;
+    exp_avg_sq_ = exp_avg_sq;
+    scale1_ = scale1.value_or(at::Tensor());
+    scale2_ = scale2.value_or(at::Tensor());
+    steps_ = steps;
+    corr_ = corr;
+    set_slots(std::move(slots));
+  }
+  std::vector<int32_t> slots() const { return slots_; }
+  void set_slots(std::vector<int32_t> s) {
+    TORCH_CHECK(s.size() == numel_.size());
+    slots_ = std::move(s);
+  }
+
+  // one step of all groups; the norm before clipping (0-dim float32) where max_norm > 0
+  std::optional<at::Tensor> step(const py::list& groups, double max_norm, double grad_mult) {
+    const at::NoGradGuard no_grad;
+    const c10::Device dev = exp_avg_.device();
+    const c10::OptionalDeviceGuard guard(dev);
+    const bool capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    std::vector<at::Tensor> keep, stepped;       // gradients laid out anew; parameters
+    std::vector<GroupWork> work;
+    std::vector<char> active(numel_.size(), 0);
+    work.reserve(groups.size());
+    int32_t at = 0;
+    for (const auto& item : groups) {
+      const py::dict group = py::reinterpret_borrow<py::dict>(item);
+      const py::list params = group["params"];
+      GroupWork w;
+      bool any = false;
+      for (const auto& obj : params) {
+        const int32_t i = at++;
+        TORCH_CHECK(THPVariable_Check(obj.ptr()) && (size_t)i < numel_.size(), "AdamW: the parameter list changed; use add_param_group");
+        const at::Tensor& p = THPVariable_Unpack(obj.ptr());
+        const at::Tensor& given = p.grad();
+        if (!given.defined()) continue;
+        TORCH_CHECK(given.layout() == at::kStrided, "AdamW does not take sparse gradients");
+        const int code = type_code(p.scalar_type());
+        TORCH_CHECK(code >= 0 && p.device() == dev && given.device() == dev && given.scalar_type() == p.scalar_type() && p.numel() == numel_[i] &&
+                        given.numel() == numel_[i] && p.is_contiguous(),
+                    "parameter ", i, " is no longer what this optimizer was built for (device, type, size or layout changed)");
+        if (numel_[i] == 0) continue;
+        const void* g = given.const_data_ptr();
+        if (!given.is_contiguous()) {
+          keep.push_back(given.contiguous());
+          g = keep.back().const_data_ptr();
+        }
+        Lists& l = w.by_type[code];
+        l.p.push_back(p.mutable_data_ptr());
+        l.g.push_back(g);
+        l.numel.push_back(numel_[i]);
+        l.first.push_back(first_[i]);
+        l.index.push_back(i);
+        active[i] = 1;
+        any = true;
+        stepped.push_back(p);
+      }
+      if (!any) continue;
+      hyper(group, dev, capturing, w);
+      work.push_back(std::move(w));
+    }
+    if (work.empty()) return std::nullopt;
+    split(active, capturing);
+    for (auto& w : work) {
+      std::vector<char> seen(numel_.size(), 0);
+      for (auto& l : w.by_type)
+        for (int32_t i : l.index) {
+          l.slot.push_back(slots_[i]);
+          if (!seen[slots_[i]]) w.slots.push_back(slots_[i]);
+          seen[slots_[i]] = 1;
+        }
+    }
+    void* stream = current_stream(dev);
+    const double* ctl = nullptr;
+    at::Tensor norm, ctl_mem, partials;
+    if (max_norm > 0.0) {
+      std::vector<std::pair<int, Lists*>> lists;
+      for (auto& w : work)
+        for (int code = 0; code < 3; ++code)
+          if (!w.by_type[code].p.empty()) lists.emplace_back(code, &w.by_type[code]);
+      partials = at::empty({Norm::partials(lists) + 2}, at::TensorOptions().dtype(at::kDouble).device(dev));
+      norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+      double* mem = partials.mutable_data_ptr<double>();       // two for the factor, then the sums
+      const int64_t count = Norm::sums(lists, mem + 2, stream);
+      check(tn_grad_norm_finish(mem + 2, count, grad_mult, max_norm, norm.mutable_data_ptr<float>(), mem, stream), "tn_grad_norm_finish");
+      ctl = mem;
+    }
+    int32_t* steps = steps_.mutable_data_ptr<int32_t>();
+    float* corr = corr_.mutable_data_ptr<float>();
+    for (auto& w : work) {
+      check(tn_adamw_tick((int32_t)w.slots.size(), w.slots.data(), steps, corr, ctl, w.lr, w.lr_dev.defined() ? w.lr_dev.const_data_ptr<float>() : nullptr,
+                          w.b1, w.b2, w.wd, stream),
+            "tn_adamw_tick");
+      for (int code = 0; code < 3; ++code) {
+        Lists& l = w.by_type[code];
+        if (l.p.empty()) continue;
+        check(tn_adamw_apply((int32_t)l.p.size(), l.p.data(), l.g.data(), l.numel.data(), l.first.data(), l.slot.data(), code, bits_,
+                             exp_avg_.mutable_data_ptr(), exp_avg_sq_.mutable_data_ptr(), scale1_.defined() ? scale1_.mutable_data_ptr<float>() : nullptr,
+                             scale2_.defined() ? scale2_.mutable_data_ptr<float>() : nullptr, blocks_, corr, ctl, grad_mult, w.b1, w.b2, w.eps, stream),
+              "tn_adamw_apply");
+      }
+    }
+    for (auto& p : stepped)
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();      // autograd has to see that the values changed
+    if (max_norm > 0.0) return norm;
+    return std::nullopt;
+  }
+
+ private:
+  void hyper(const py::dict& group, const c10::Device& dev, bool capturing, GroupWork& w) {
+    const py::object lr = group["lr"];
+    w.lr = 0.0;
+    if (THPVariable_Check(lr.ptr())) {
+      w.lr_dev = THPVariable_Unpack(lr.ptr());
+      TORCH_CHECK_VALUE(w.lr_dev.scalar_type() == at::kFloat && w.lr_dev.dim() == 0 && w.lr_dev.device() == dev,
+                        "a tensor lr must be a 0-dim float32 tensor on the parameters' device");
+    } else {
+      TORCH_CHECK(!capturing, "AdamW: give lr as a 0-dim device tensor to capture a step (a number would be frozen into the graph)");
+      w.lr = lr.cast<double>();
+      TORCH_CHECK_VALUE(w.lr >= 0.0, "Invalid learning rate: ", w.lr);
+    }
+    const py::sequence betas = group["betas"];
+    w.b1 = betas[0].cast<double>();
+    w.b2 = betas[1].cast<double>();
+    w.eps = group["eps"].cast<double>();
+    w.wd = group["weight_decay"].cast<double>();
+    TORCH_CHECK_VALUE(w.b1 >= 0.0 && w.b1 < 1.0 && w.b2 >= 0.0 && w.b2 < 1.0, "betas must be two numbers in [0, 1)");
+    TORCH_CHECK_VALUE(w.eps >= 0.0 && w.wd >= 0.0, "eps and weight_decay must not be negative");
+  }
+
+  // Step counts belong to slots.  Where some of a slot's tensors have a gradient and others have not, those that have get a slot of
+  // their own, starting at the same count.  (There are as many slots as tensors, so one is free whenever two tensors share one.)
+  void split(const std::vector<char>& active, bool capturing) {
+    const size_t n = slots_.size();
+    std::vector<int32_t> some(n, 0), every(n, 0);
+    for (size_t i = 0; i < n; ++i) {
+      if (numel_[i] == 0) continue;
+      every[slots_[i]]++;
+      some[slots_[i]] += active[i];
+    }
+    for (size_t s = 0; s < n; ++s) {
+      if (some[s] == 0 || some[s] == every[s]) continue;
+      TORCH_CHECK(!capturing, "AdamW: other parameters than before have gradients in a captured step: run such a step once before capturing it");
+      std::vector<char> used(n, 0);
+      for (int32_t k : slots_) used[k] = 1;
+      size_t free = 0;
+      while (used[free]) ++free;
+      steps_.narrow(0, (int64_t)free, 1).copy_(steps_.narrow(0, (int64_t)s, 1));
+      for (size_t i = 0; i < n; ++i)
+        if (slots_[i] == (int32_t)s && active[i]) slots_[i] = (int32_t)free;
+    }
+  }
+
+  int bits_;
+  int64_t blocks_ = 0;
+  std::vector<int64_t> numel_, first_;
+  std::vector<int32_t> slots_;
+  at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_;
+};
+
+at::Tensor grad_norm(const std::vector<at::Tensor>& tensors) {
+  const at::NoGradGuard no_grad;
+  TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm needs at least one tensor");
+  const c10::Device dev = tensors[0].device();
+  for (const auto& t : tensors) {
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided && type_code(t.scalar_type()) >= 0, "grad_norm takes dense float32, bfloat16 or float16 tensors");
+    TORCH_CHECK(t.is_cuda(), "titanet_amd.optim needs ROCm device tensors; there is no CPU execution path");
+    TORCH_CHECK_VALUE(t.device() == dev, "grad_norm takes tensors of one device, got ", dev, " and ", t.device());
+  }
+  const c10::OptionalDeviceGuard guard(dev);
+  std::vector<at::Tensor> keep;
+  std::array<Lists, 3> by_type;
+  for (const auto& t : tensors) {
+    keep.push_back(t.is_contiguous() ? t : t.contiguous());
+    Lists& l = by_type[type_code(t.scalar_type())];
+    l.g.push_back(keep.back().const_data_ptr());
+    l.numel.push_back(t.numel());
+  }
+  std::vector<std::pair<int, Lists*>> lists;
+  for (int code = 0; code < 3; ++code)
+    if (!by_type[code].g.empty()) lists.emplace_back(code, &by_type[code]);
+  void* stream = current_stream(dev);
+  at::Tensor partials = at::empty({Norm::partials(lists) + 1}, at::TensorOptions().dtype(at::kDouble).device(dev));
+  at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+  const int64_t count = Norm::sums(lists, partials.mutable_data_ptr<double>(), stream);
+  check(tn_grad_norm_finish(partials.const_data_ptr<double>(), count, 1.0, INFINITY, norm.mutable_data_ptr<float>(), nullptr, stream), "tn_grad_norm_finish");
+  return norm;
+}
+
+// --------------------------------------------------------------------------------------------------------- 8-bit product
+std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& given) {
+  const at::NoGradGuard no_grad;
+  TORCH_CHECK_TYPE(type_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "quantize_rows takes a float32, bfloat16 or float16 matrix, got ", given.scalar_type());
+  TORCH_CHECK_VALUE(given.dim() == 2 && given.size(1) >= 1, "quantize_rows takes a matrix with at least one column, got ", given.sizes());
+  TORCH_CHECK_VALUE(given.size(1) <= TN_INT8_MAX_K, "rows of more than ", TN_INT8_MAX_K, " values could overflow the 32-bit sums");
+  TORCH_CHECK(given.is_cuda(), "titanet_amd.int8: x must be a ROCm device tensor; there is no CPU execution path");
+  const c10::OptionalDeviceGuard guard(given.device());
+  const at::Tensor x = given.stride(1) == 1 || given.size(1) == 1 ? given : given.contiguous();
+  const int64_t rows = x.size(0), cols = x.size(1), ld = (cols + 63) / 64 * 64;
+  at::Tensor codes = at::empty({rows, ld}, x.options().dtype(at::kChar)), scales = at::empty({rows}, x.options().dtype(at::kFloat));
+  check(tn_int8_quantize_rows(x.const_data_ptr(), type_code(x.scalar_type()), rows, cols, x.stride(0), codes.mutable_data_ptr(), ld,
+                              scales.mutable_data_ptr<float>(), current_stream(x.device())),
+        "tn_int8_quantize_rows");
+  return {codes, scales};
+}
+
+struct Out {
+  at::Tensor bias, y;
+  const float* bias_ptr = nullptr;
+};
+
+Out prepare_out(const c10::Device& dev, int64_t cols_a, int64_t cols, int64_t m, const at::Tensor& b, const std::optional<at::Tensor>& bias,
+                c10::ScalarType out) {
+  TORCH_CHECK_TYPE(type_code(out) >= 0, "out_dtype must be float32, bfloat16 or float16, got ", out);
+  TORCH_CHECK_VALUE(cols_a == cols, "operands of ", cols_a, " and ", cols, " columns");
+  TORCH_CHECK_VALUE(dev == b.device(), "operands on different devices: ", dev, " and ", b.device());
+  Out o;
+  const int64_t n = b.size(0);
+  if (bias) {
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == n && bias->device() == b.device(), "bias must be float32 [", n, "] on ",
+                      b.device(), ", got ", bias->scalar_type(), " ", bias->sizes(), " on ", bias->device());
+    o.bias = bias->is_contiguous() ? *bias : bias->contiguous();
+    o.bias_ptr = o.bias.const_data_ptr<float>();
+  }
+  o.y = at::empty({m, n}, b.options().dtype(out));
+  return o;
+}
+
+void product(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols, Out& o) {
+  check(tn_int8_matmul(a.const_data_ptr(), a_scales.const_data_ptr<float>(), a.size(1), b.const_data_ptr(), b_scales.const_data_ptr<float>(), b.size(1),
+                       o.bias_ptr, o.y.mutable_data_ptr(), type_code(o.y.scalar_type()), b.size(0), a.size(0), b.size(0), cols, current_stream(b.device())),
+        "tn_int8_matmul");
+}
+
+at::Tensor matmul_rows(const at::Tensor& a, const at::Tensor& a_scales, int64_t cols_a, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols,
+                       const std::optional<at::Tensor>& bias, std::optional<c10::ScalarType> out) {
+  const c10::OptionalDeviceGuard guard(b.device());
+  TORCH_CHECK(!(at::GradMode::is_enabled() && bias && bias->requires_grad()), "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
+  const at::NoGradGuard no_grad;
+  Out o = prepare_out(a.device(), cols_a, cols, a.size(0), b, bias, out.value_or(at::kFloat));
+  product(a, a_scales, b, b_scales, cols, o);
+  return o.y;
+}
+
+at::Tensor matmul_float(const at::Tensor& x, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols, const std::optional<at::Tensor>& bias,
+                        std::optional<c10::ScalarType> out) {
+  TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0 && x.layout() == at::kStrided,
+                   "the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1, "the first operand needs at least one dimension");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias && bias->requires_grad()))),
+              "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
+  const at::NoGradGuard no_grad;
+  const c10::OptionalDeviceGuard guard(b.device());
+  const int64_t cols_a = x.size(-1);
+  TORCH_CHECK_VALUE(cols_a == cols, "operands of ", cols_a, " and ", cols, " columns");
+  const at::Tensor flat = x.dim() == 2 ? x : x.reshape({-1, cols});
+  Out o = prepare_out(x.device(), cols_a, cols, flat.size(0), b, bias, out.value_or(x.scalar_type()));
+  auto [codes, scales] = quantize_rows(flat);
+  product(codes, scales, b, b_scales, cols, o);
+  if (x.dim() == 2) return o.y;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = b.size(0);
+  return o.y.view(shape);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_host, m) {
+  py::class_<Stepper>(m, "Stepper")
+      .def(py::init<int>())
+      .def("layout", &Stepper::layout)
+      .def("step", &Stepper::step)
+      .def_property("slots", &Stepper::slots, &Stepper::set_slots);
+  m.def("grad_norm", &grad_norm);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("matmul_rows", &matmul_rows);
+  m.def("matmul_float", &matmul_float);
+}

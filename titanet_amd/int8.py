@@ -9,20 +9,12 @@ src/learn.py:441-447).  Here both operands are int8 rows with one float32 scale 
 (``tn_int8_matmul``, include/titanet_amd.h) and one multiplication by both scales follows.  For serving: there is no backward
 pass and no CPU fallback.
 """
-import ctypes as C
-
 import torch
 import torch.nn as nn
 
 from . import _lib
-from ._lib import check
 
 MAX_K = 131071       # TN_INT8_MAX_K: 128 * 128 * MAX_K still fits 32 bits
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _p(t):
-    return C.c_void_p(t.data_ptr() if t is not None else 0)
 
 
 def _need_device(t, what):
@@ -78,23 +70,10 @@ class Int8Rows:
 def quantize_rows(x):
     """``Int8Rows`` of a float matrix (float32, bfloat16 or float16): scale max |row| / 127 (at least 2^-126; 0 for a row of
     zeros), codes the nearest integers to x / scale, even half way.  A row with a NaN or an infinity gets the scale NaN."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
-        raise TypeError(f"quantize_rows takes a float32, bfloat16 or float16 matrix, got {getattr(x, 'dtype', type(x))}")
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"quantize_rows takes a matrix with at least one column, got {tuple(x.shape)}")
-    if x.shape[1] > MAX_K:
-        raise ValueError(f"rows of more than {MAX_K} values could overflow the 32-bit sums")
-    _need_device(x, "x")
-    x = x.detach()
-    if x.stride(1) != 1 or x.stride(0) < 0:
-        x = x.contiguous()
-    rows, cols = x.shape
-    with torch.cuda.device(x.device):
-        padded = torch.empty(rows, (cols + 63) // 64 * 64, dtype=torch.int8, device=x.device)
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-        check(_lib.load().tn_int8_quantize_rows(_p(x), _TYPES[x.dtype], rows, cols, x.stride(0), _p(padded), padded.shape[1], _p(scales),
-                                                C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)), "tn_int8_quantize_rows")
-    return Int8Rows._of(padded, scales, cols)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"quantize_rows takes a float32, bfloat16 or float16 matrix, got {type(x).__name__}")
+    padded, scales = _lib.load_host().quantize_rows(x)
+    return Int8Rows._of(padded, scales, x.shape[1])
 
 
 def int8_matmul(a, b, bias=None, out_dtype=None):
@@ -104,37 +83,10 @@ def int8_matmul(a, b, bias=None, out_dtype=None):
     if not isinstance(b, Int8Rows):
         raise TypeError(f"the second operand must be Int8Rows (quantize_rows), got {type(b).__name__}")
     if isinstance(a, torch.Tensor):
-        if a.dtype not in _TYPES:
-            raise TypeError(f"the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got {a.dtype}")
-        if a.dim() < 1:
-            raise ValueError("the first operand needs at least one dimension")
-        if torch.is_grad_enabled() and (a.requires_grad or (bias is not None and bias.requires_grad)):
-            raise RuntimeError("int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()")
-        lead, cols, dtype = a.shape[:-1], a.shape[-1], a.dtype
-    elif isinstance(a, Int8Rows):
-        lead, cols, dtype = (len(a),), a.cols, torch.float32
-    else:
-        raise TypeError(f"the first operand must be Int8Rows or a tensor, got {type(a).__name__}")
-    out_dtype = dtype if out_dtype is None else out_dtype
-    if out_dtype not in _TYPES:
-        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    if cols != b.cols:
-        raise ValueError(f"operands of {cols} and {b.cols} columns")
-    if a.device != b.device:
-        raise ValueError(f"operands on different devices: {a.device} and {b.device}")
-    if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (len(b),) or bias.device != b.device:
-            raise ValueError(f"bias must be float32 [{len(b)}] on {b.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-        bias = bias.detach().contiguous()
-    if isinstance(a, torch.Tensor):
-        a = quantize_rows(a.detach().reshape(-1, cols))
-    m, n = len(a), len(b)
-    with torch.cuda.device(b.device):
-        y = torch.empty(m, n, dtype=out_dtype, device=b.device)
-        check(_lib.load().tn_int8_matmul(_p(a._padded), _p(a.scales), a._padded.shape[1], _p(b._padded), _p(b.scales), b._padded.shape[1],
-                                         _p(bias), _p(y), _TYPES[out_dtype], n, m, n, cols,
-                                         C.c_void_p(torch.cuda.current_stream(b.device).cuda_stream)), "tn_int8_matmul")
-    return y.view(*lead, n)
+        return _lib.load_host().matmul_float(a, b._padded, b.scales, b.cols, bias, out_dtype)
+    if isinstance(a, Int8Rows):
+        return _lib.load_host().matmul_rows(a._padded, a.scales, a.cols, b._padded, b.scales, b.cols, bias, out_dtype)
+    raise TypeError(f"the first operand must be Int8Rows or a tensor, got {type(a).__name__}")
 
 
 class Int8Linear(nn.Module):

@@ -21,60 +21,14 @@ BLOCK = 256          # TN_OPT_BLOCK: elements that share a scale of the 8-bit mo
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _at(array):
-    return array.ctypes.data_as(C.c_void_p)          # (keeps the array alive as long as the pointer)
-
-
 def _dev(tensor):
     return C.c_void_p(tensor.data_ptr() if tensor is not None else 0)
-
-
-def _pointers(tensors):
-    return np.array([t.data_ptr() for t in tensors], dtype=np.uint64)
-
-
-def _sumsq(lib, tensors, partials, at, stream):
-    """partial sums of squares of ``tensors`` (contiguous, one device) into ``partials`` from ``at`` on; returns where they end"""
-    written = C.c_int64()
-    for dtype, code in _TYPES.items():
-        some = [t for t in tensors if t.dtype is dtype]
-        if not some:
-            continue
-        numel = np.array([t.numel() for t in some], dtype=np.int64)
-        check(lib.tn_grad_sumsq(len(some), _at(_pointers(some)), _at(numel), code, C.c_void_p(partials.data_ptr() + 8 * at),
-                                C.byref(written), C.c_void_p(stream)), "tn_grad_sumsq")
-        at += written.value
-    return at
-
-
-def _partials(lib, tensors, device):
-    numel = np.array([t.numel() for t in tensors], dtype=np.int64)
-    return torch.empty(max(1, int(lib.tn_grad_sumsq_partials(len(tensors), _at(numel)))), dtype=torch.float64, device=device)
 
 
 def grad_norm(tensors):
     """The 2-norm of all elements of ``tensors`` together, as a 0-dim float32 tensor on their device.  Summed in 64 bits in a
     fixed order: two calls on the same values give the same number.  float32, bfloat16 and float16 may be mixed."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not tensors:
-        raise ValueError("grad_norm needs at least one tensor")
-    device = tensors[0].device
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _TYPES:
-            raise TypeError("grad_norm takes dense float32, bfloat16 or float16 tensors")
-        if not t.is_cuda:
-            raise RuntimeError("titanet_amd.optim needs ROCm device tensors; there is no CPU execution path")
-        if t.device != device:
-            raise ValueError(f"grad_norm takes tensors of one device, got {device} and {t.device}")
-    lib = _lib.load()
-    with torch.no_grad(), torch.cuda.device(device):
-        tensors = [t.detach().contiguous() for t in tensors]
-        stream = torch.cuda.current_stream(device).cuda_stream
-        partials, norm = _partials(lib, tensors, device), torch.empty((), dtype=torch.float32, device=device)
-        count = _sumsq(lib, tensors, partials, 0, stream)
-        check(lib.tn_grad_norm_finish(_dev(partials), count, 1.0, float("inf"), _dev(norm), C.c_void_p(0), C.c_void_p(stream)),
-              "tn_grad_norm_finish")
-    return norm
+    return _lib.load_host().grad_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -105,10 +59,10 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.grad_mult = state_bits, max_grad_norm, float(grad_mult)
         self.last_grad_norm = None
         self._native = _lib.load()
+        self._stepper = _lib.load_host().Stepper(state_bits)      # checks, collects and launches a step
         self._list, self._device = [], None          # all parameters, group after group
         self._exp_avg = self._exp_avg_sq = self._scale1 = self._scale2 = self._steps = self._corr = None
         self._numel = self._first = np.zeros(0, dtype=np.int64)
-        self._slots = np.zeros(0, dtype=np.int32)
         self.blocks = 0
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
@@ -173,7 +127,7 @@ class AdamW(torch.optim.Optimizer):
         self._list += new
         self._numel, self._first = np.concatenate([self._numel, numel]), np.concatenate([self._first, first])
         # one step count for the whole group until some of its tensors go without a gradient
-        self._slots = np.concatenate([self._slots, np.full(len(new), n0, dtype=np.int32)])
+        slots = self._stepper.slots + [n0] * len(new)
         self.blocks = b0 + int(blocks.sum())
 
         def grown(old, size, dtype):
@@ -188,6 +142,8 @@ class AdamW(torch.optim.Optimizer):
             self._scale1, self._scale2 = grown(self._scale1, self.blocks, torch.float32), grown(self._scale2, self.blocks, torch.float32)
         self._steps = grown(self._steps, len(self._list), torch.int32)
         self._corr = torch.zeros(len(self._list), 4, dtype=torch.float32, device=self._device)
+        self._stepper.layout(self._numel.tolist(), self._first.tolist(), slots, self.blocks, self._exp_avg, self._exp_avg_sq, self._scale1,
+                             self._scale2, self._steps, self._corr)
 
     def _groups(self):
         """(group, index of its first parameter) in order"""
@@ -197,88 +153,15 @@ class AdamW(torch.optim.Optimizer):
             at += len(group["params"])
 
     # ------------------------------------------------------------------ the step
-    def _collect(self, group, at):
-        """[(index, parameter, gradient)] of the parameters of a group that have one"""
-        active = []
-        for i, p in enumerate(group["params"], at):
-            g = p.grad
-            if g is None:
-                continue
-            if g.layout != torch.strided:
-                raise RuntimeError("AdamW does not take sparse gradients")
-            if p.device != self._device or g.device != self._device or p.dtype != g.dtype or p.numel() != self._numel[i] or not p.is_contiguous():
-                raise RuntimeError(f"parameter {i} is no longer what this optimizer was built for (device, size or layout changed)")
-            if p.numel():
-                active.append((i, p, g if g.is_contiguous() else g.contiguous()))
-        return active
-
-    def _split(self, index, capturing):
-        """Step counts belong to slots.  Where some of a slot's tensors have a gradient and others have not, those that have get a
-        slot of their own, starting at the same count."""
-        slots = self._slots
-        active = np.zeros(len(slots), dtype=bool)
-        active[index] = True
-        for s in np.unique(slots[index]):
-            rest = (slots == s) & ~active
-            if not rest.any():
-                continue
-            if capturing:
-                raise RuntimeError("AdamW: other parameters than before have gradients in a captured step: run such a step once before capturing it")
-            free = int(np.setdiff1d(np.arange(len(slots)), slots)[0])
-            self._steps[free:free + 1].copy_(self._steps[int(s):int(s) + 1])
-            slots[(slots == s) & active] = free
-        return np.unique(slots[index]).astype(np.int32)
-
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._device is None:
-            return loss
-        with torch.no_grad(), torch.cuda.device(self._device):
-            self._step()
+        if self._device is not None:
+            norm = self._stepper.step(self.param_groups, 0.0 if self.max_grad_norm is None else float(self.max_grad_norm), self.grad_mult)
+            self.last_grad_norm = self.last_grad_norm if norm is None else norm
         return loss
-
-    def _step(self):
-        lib, vp = self._native, C.c_void_p
-        capturing = torch.cuda.is_current_stream_capturing()
-        work = []
-        for group, at in self._groups():
-            active = self._collect(group, at)
-            if not active:
-                continue
-            self._check_hyper(group)
-            if capturing and not isinstance(group["lr"], torch.Tensor):
-                raise RuntimeError("AdamW: give lr as a 0-dim device tensor to capture a step (a number would be frozen into the graph)")
-            work.append((group, active, self._split(np.array([a[0] for a in active]), capturing)))
-        if not work:
-            return
-        stream = torch.cuda.current_stream(self._device).cuda_stream
-        ctl = None
-        if self.max_grad_norm is not None:
-            grads = [a[2] for _, active, _ in work for a in active]
-            partials = _partials(lib, grads, self._device)
-            count = _sumsq(lib, grads, partials, 0, stream)
-            ctl = torch.empty(2, dtype=torch.float64, device=self._device)
-            self.last_grad_norm = torch.empty((), dtype=torch.float32, device=self._device)
-            check(lib.tn_grad_norm_finish(_dev(partials), count, self.grad_mult, float(self.max_grad_norm), _dev(self.last_grad_norm),
-                                          _dev(ctl), vp(stream)), "tn_grad_norm_finish")
-        for group, active, slots in work:
-            lr, (b1, b2) = group["lr"], group["betas"]
-            lr_dev = lr if isinstance(lr, torch.Tensor) else None
-            check(lib.tn_adamw_tick(len(slots), _at(slots), _dev(self._steps), _dev(self._corr), _dev(ctl), 0.0 if lr_dev is not None else float(lr),
-                                    _dev(lr_dev), b1, b2, group["weight_decay"], vp(stream)), "tn_adamw_tick")
-            for dtype, code in _TYPES.items():
-                some = [a for a in active if a[1].dtype is dtype]
-                if not some:
-                    continue
-                index = np.array([a[0] for a in some])
-                check(lib.tn_adamw_apply(len(some), _at(_pointers([a[1] for a in some])), _at(_pointers([a[2] for a in some])),
-                                         _at(self._numel[index]), _at(self._first[index]), _at(self._slots[index]), code, self.state_bits,
-                                         _dev(self._exp_avg), _dev(self._exp_avg_sq), _dev(self._scale1), _dev(self._scale2), self.blocks,
-                                         _dev(self._corr), _dev(ctl), self.grad_mult, b1, b2, group["eps"], vp(stream)), "tn_adamw_apply")
-            torch.autograd.graph.increment_version([a[1] for a in active])
 
     # ------------------------------------------------------------------ moments as values
     def moments(self):
@@ -323,12 +206,13 @@ class AdamW(torch.optim.Optimizer):
 
     def _put_steps(self, steps):
         """one slot for each group and count"""
-        slot_of, counts = {}, torch.zeros(len(self._list), dtype=torch.int32)
+        slot_of, slots, counts = {}, [0] * len(self._list), torch.zeros(len(self._list), dtype=torch.int32)
         for k, (group, at) in enumerate(self._groups()):
             for i in range(at, at + len(group["params"])):
                 s = slot_of.setdefault((k, steps[i]), i)
-                self._slots[i] = s
+                slots[i] = s
                 counts[s] = steps[i]
+        self._stepper.slots = slots
         self._steps.copy_(counts)
 
     # ------------------------------------------------------------------ checkpoints
@@ -345,12 +229,12 @@ class AdamW(torch.optim.Optimizer):
         """``torch.optim.AdamW``'s layout, the moments as they are held: float32, or int8 / uint8 codes with ``exp_avg_scale`` /
         ``exp_avg_sq_scale`` per block of 256 elements.  Parameters that were never stepped have no entry."""
         state, groups = {}, []
-        counts = self._steps.cpu().tolist() if self._device is not None else []
+        counts, slots = (self._steps.cpu().tolist(), self._stepper.slots) if self._device is not None else ([], [])
         for group, at in self._groups():
             index = list(range(at, at + len(group["params"])))
             groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": index})
             for i in index:
-                t = counts[self._slots[i]]
+                t = counts[slots[i]]
                 if t:
                     state[i] = {"step": torch.tensor(float(t)), **self._views(i)}
         return {"state": state, "param_groups": groups}
