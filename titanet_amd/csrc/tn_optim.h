@@ -74,22 +74,30 @@ __device__ __forceinline__ float opt_max_wave(float x) {
 // The nearest code is decided in 64 bits (vector double arithmetic runs at the rate of single here, and the kernels wait for
 // memory): the code of a value is then a matter of the definition, not of a kernel's rounding.  The candidate c comes from a
 // single-precision root, at most one below; one comparison with the border (c + 1/2) settles it, half way goes to the lower.
+// The largest value is worth its scale exactly (16129 * fl(1 / 16129) = 1, 255^4 likewise), and opt_ema rounds each product and
+// the sum as written: with b1 = 9/10 one new scale in a hundred lies half way between two floats, where a fused
+// multiply-add would turn it the other way than the same formula computed elsewhere.
 // A block that holds a NaN or an infinity gets the scale NaN: all its values are NaN then, and stay so.
 __device__ __forceinline__ void opt_decode_first(uint32_t q, float scale, double x[4]) {
-  const double s = (double)scale * (1.0 / 16129.0);
+  const double s = (double)scale;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int c = (int8_t)(q >> (8 * j));
-    x[j] = (double)(c < 0 ? -c * c : c * c) * s;
+    x[j] = ((double)(c < 0 ? -c * c : c * c) * (1.0 / 16129.0)) * s;
   }
 }
 __device__ __forceinline__ void opt_decode_second(uint32_t q, float scale, double x[4]) {
-  const double s = (double)scale * (1.0 / 4228250625.0);      // 255^4
+  const double s = (double)scale;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t c = (q >> (8 * j)) & 255u;
-    x[j] = (double)(c * c * c * c) * s;                         // below 2^32
+    x[j] = ((double)(c * c * c * c) * (1.0 / 4228250625.0)) * s;      // 255^4, below 2^32
   }
+}
+__device__ __forceinline__ double opt_ema(double b, double x, double w, double y) {
+#pragma clang fp contract(off)
+  const double p = b * x, q = w * y;
+  return p + q;
 }
 // all 64 lanes of the wave call these, each with four of the block's 256 values; *scale is that of the block, infinity or NaN
 // if one of its values is

@@ -177,8 +177,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double gj = (double)gv[j] * factor;
-      m[j] = h.b1 * m[j] + h.w1 * gj;
-      v[j] = h.b2 * v[j] + h.w2 * (gj * gj);
+      m[j] = opt_ema(h.b1, m[j], h.w1, gj);
+      v[j] = opt_ema(h.b2, v[j], h.w2, gj * gj);
       pv[j] = pv[j] * c.z - c.x * ((float)m[j] / (sqrtf((float)v[j]) * c.y + h.eps));
     }
     opt_store4(p, i, n, pv);
