@@ -246,6 +246,12 @@ int tn_int8_quantize_rows(const void* x, int32_t dtype, int64_t rows, int64_t co
                           float* scales, void* stream);
 int tn_int8_matmul(const void* a, const float* a_scales, int64_t lda, const void* b, const float* b_scales, int64_t ldb, const float* bias,
                    void* y, int32_t y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, void* stream);
+/* The same from float rows x [m][ldx], quantised on the way.  workspace: 16-byte aligned device memory of at least
+ * tn_int8_linear_workspace(m, k) bytes, not read after the call's kernels; 0 (a few rows, quantised inside the product): may be NULL. */
+int64_t tn_int8_linear_workspace(int64_t m, int64_t k);
+int tn_int8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* b, const float* b_scales, int64_t ldb, const float* bias,
+                   void* y, int32_t y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 
 /* ---- stand-alone loss heads: MetricLearningLoss.forward(inputs, targets) -> (normalised inputs, preds, loss)
  * (reference src/losses.py:32-44 CELoss, :77-132 AngularMarginLoss) for callers that use a loss object outside

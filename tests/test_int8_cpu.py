@@ -51,3 +51,12 @@ def test_c_entries_refuse_before_they_touch_the_device():
     assert matmul(a=none) == bad and matmul(y=none) == bad and matmul(b=C.c_void_p(4097)) == bad
     assert matmul(lda=32) == bad and matmul(k=65) == bad and matmul(ldy=4) == bad
     assert matmul(dtype=-1) == unsupported and matmul(lda=131072, ldb=131072, k=131072) == unsupported
+
+    def linear(x=at, xd=0, yd=0, m=4, ws=none, size=0, ldx=3, ldb=64):
+        return lib.tn_int8_linear(x, xd, ldx, at, at, ldb, none, at, yd, 5, m, 5, 3, ws, size, none)
+
+    assert linear(m=0) == 0 and linear(x=none) == bad and linear(ldx=-1) == bad and linear(ldb=63) == bad
+    assert linear(xd=5) == unsupported and linear(yd=5) == unsupported
+    need = lib.tn_int8_linear_workspace(100, 3)
+    assert need == 100 * 64 + 400 and lib.tn_int8_linear_workspace(4, 3) == 0 and lib.tn_int8_linear_workspace(4, 0) == bad
+    assert linear(m=100) == bad and linear(m=100, ws=at, size=need - 1) == bad and linear(m=100, ws=C.c_void_p(4104), size=need) == bad

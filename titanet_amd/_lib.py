@@ -21,6 +21,7 @@ EXPORTS = [
     "tn_forward_masked", "tn_forward_prepacked", "tn_plan_prolog_input", "tn_mel_forward_batch_packed", "tn_plan_set_grad_groups", "tn_plan_num_grad_buckets", "tn_plan_grad_bucket", "tn_plan_wait_grad_bucket",
     "tn_mark_host", "tn_grad_sumsq_partials", "tn_grad_sumsq", "tn_grad_norm_finish", "tn_adamw_tick", "tn_adamw_apply", "tn_moments_decode",
     "tn_moments_encode", "tn_int8_quantize_rows", "tn_int8_matmul",
+    "tn_int8_linear_workspace", "tn_int8_linear",
 ]
 
 
@@ -116,6 +117,9 @@ def load():
     lib.tn_moments_encode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
     lib.tn_int8_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]
     lib.tn_int8_matmul.argtypes = [vp, vp, i64, vp, vp, i64, vp, vp, i32, i64, i64, i64, i64, vp]
+    lib.tn_int8_linear_workspace.argtypes = [i64, i64]
+    lib.tn_int8_linear_workspace.restype = i64
+    lib.tn_int8_linear.argtypes = [vp, i32, i64, vp, vp, i64, vp, vp, i32, i64, i64, i64, i64, vp, i64, vp]
     lib.tn_version.restype = C.c_char_p
     for name in EXPORTS:
         fn = getattr(lib, name)

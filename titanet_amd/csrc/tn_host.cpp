@@ -330,8 +330,14 @@ at::Tensor matmul_float(const at::Tensor& x, const at::Tensor& b, const at::Tens
   TORCH_CHECK_VALUE(cols_a == cols, "operands of ", cols_a, " and ", cols, " columns");
   const at::Tensor flat = x.dim() == 2 ? x : x.reshape({-1, cols});
   Out o = prepare_out(x.device(), cols_a, cols, flat.size(0), b, bias, out.value_or(x.scalar_type()));
-  auto [codes, scales] = quantize_rows(flat);
-  product(codes, scales, b, b_scales, cols, o);
+  const at::Tensor rows = flat.stride(1) == 1 || cols == 1 ? flat : flat.contiguous();
+  const int64_t bytes = tn_int8_linear_workspace(rows.size(0), cols);
+  at::Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, b.options());
+  check(tn_int8_linear(rows.const_data_ptr(), type_code(x.scalar_type()), rows.stride(0), b.const_data_ptr(), b_scales.const_data_ptr<float>(), b.size(1),
+                       o.bias_ptr, o.y.mutable_data_ptr(), type_code(o.y.scalar_type()), b.size(0), rows.size(0), b.size(0), cols,
+                       bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, current_stream(b.device())),
+        "tn_int8_linear");
   if (x.dim() == 2) return o.y;
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = b.size(0);

@@ -34,26 +34,87 @@ __device__ __forceinline__ int q8_code(float x, float s, float inv) {
 
 __device__ __forceinline__ float q8_scale(float top) { return top > 0.f ? fmaxf(top / 127.f, 0x1p-126f) : 0.f; }
 
-// one wave per row: maximum, then codes
+__device__ __forceinline__ float q8_max_group(float x, int group) {       // over aligned groups of `group` lanes
+  for (int d = group >> 1; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+  return x;
+}
+
+// eight consecutive elements from k on as floats, zeros behind the row's end; the type's own alignment is enough
 template <typename T>
+struct Q8Vec {
+  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+template <typename T>
+__device__ __forceinline__ void q8_load8(const T* row, int k, int cols, float v[8]) {
+  if (k + 8 <= cols) {
+    const typename Q8Vec<T>::type x = *reinterpret_cast<const typename Q8Vec<T>::type*>(row + k);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)x[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? (float)row[k + j] : 0.f;
+  }
+}
+// largest |v|, NaN where one of them is not finite (a later maximum then has to look for it: fmaxf drops NaN)
+__device__ __forceinline__ float q8_top8(const float v[8], float top, bool& bad) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bad |= !(fabsf(v[j]) < __builtin_huge_valf());
+  return top;
+}
+__device__ __forceinline__ uint2 q8_pack8(const float v[8], float s, float inv) {
+  uint2 q = make_uint2(0u, 0u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    q.x |= (uint32_t)(uint8_t)q8_code(v[j], s, inv) << (8 * j);
+    q.y |= (uint32_t)(uint8_t)q8_code(v[4 + j], s, inv) << (8 * j);
+  }
+  return q;
+}
+
+// Codes and scale of every row.  A row belongs to GROUP lanes of a wave, eight elements to a lane and pass, kept in registers
+// between the maximum and the codes where PASSES of them hold the row (PASSES = 0: read twice).  One pass over memory; what
+// bounds it is HBM.
+template <typename T, int GROUP, int PASSES>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ q,
-                                                            int64_t ldq, float* __restrict__ scales) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+                                                            int64_t ldq, int padded, float* __restrict__ scales) {
+  constexpr int PER = 64 / GROUP;                  // rows of a wave
+  const int lane = threadIdx.x & 63, in = lane % GROUP;
+  for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * PER; r0 < rows; r0 += (int64_t)gridDim.x * 4 * PER) {
+    const int64_t r = r0 + lane / GROUP < rows ? r0 + lane / GROUP : rows - 1;       // (the last row twice: the same codes)
     const T* row = x + r * ldx;
+    float v[PASSES ? PASSES : 1][8];
     float top = 0.f;
     bool bad = false;
-    for (int k = lane; k < cols; k += 64) {
-      const float a = fabsf((float)row[k]);
-      bad |= !(a < __builtin_huge_valf());
-      top = fmaxf(top, a);
-    }
+    if constexpr (PASSES > 0) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    bad = __ballot(bad) != 0;
-    const float s = q8_scale(top), inv = s > 0.f ? 1.f / s : 0.f;
-    for (int64_t k = lane; k < ldq; k += 64) q[r * ldq + k] = !bad && s > 0.f && k < cols ? (int8_t)q8_code((float)row[k], s, inv) : (int8_t)0;
-    if (lane == 0) scales[r] = bad ? __builtin_nanf("") : s;
+      for (int p = 0; p < PASSES; ++p) q8_load8(row, (p * GROUP + in) * 8, cols, v[p]);
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) top = q8_top8(v[p], top, bad);
+    } else {
+      for (int k = in * 8; k < cols; k += GROUP * 8) {
+        q8_load8(row, k, cols, v[0]);
+        top = q8_top8(v[0], top, bad);
+      }
+    }
+    top = q8_max_group(bad ? __builtin_huge_valf() : top, GROUP);
+    const bool finite = top < __builtin_huge_valf();
+    const float s = finite ? q8_scale(top) : 0.f, inv = s > 0.f ? 1.f / s : 0.f;
+    uint2* out = reinterpret_cast<uint2*>(q + r * ldq);
+    if constexpr (PASSES > 0) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int k = (p * GROUP + in) * 8;
+        if (k < padded) out[k / 8] = s > 0.f ? q8_pack8(v[p], s, inv) : make_uint2(0u, 0u);
+      }
+    } else {
+      for (int k = in * 8; k < padded; k += GROUP * 8) {
+        q8_load8(row, k, cols, v[0]);
+        out[k / 8] = s > 0.f ? q8_pack8(v[0], s, inv) : make_uint2(0u, 0u);
+      }
+    }
+    if (in == 0) scales[r] = finite ? s : __builtin_nanf("");
   }
 }
 
@@ -65,52 +126,258 @@ struct Int8Args {
   int k;                              // multiple of 64
 };
 
-// 128 x 128 outputs per workgroup, 64 x 64 per wave (2 x 2 matrix instructions of 32 x 32 x 32), K in steps of 64 bytes through LDS
 template <typename T>
-__global__ __launch_bounds__(256) void int8_matmul_kernel(Int8Args g, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) int8_t ta[128 * 80], tb[128 * 80];       // rows of 64 bytes, padded to 80
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * 128, n0 = (int64_t)(blockIdx.x % tiles_n) * 128;
-  i32x16_t acc[2][2] = {};
-  const int row = tid >> 1, part = (tid & 1) * 32;
-  const int64_t ra = std::min<int64_t>(m0 + row, g.m - 1), rb = std::min<int64_t>(n0 + row, g.n - 1);
-  const int8_t *pa = g.a + ra * g.lda + part, *pb = g.b + rb * g.ldb + part;
-  const int fi = lane & 31, fh = lane >> 5;
-  for (int k = 0; k < g.k; k += 64) {
-    const i32x4_t a0 = *reinterpret_cast<const i32x4_t*>(pa + k), a1 = *reinterpret_cast<const i32x4_t*>(pa + k + 16);
-    const i32x4_t b0 = *reinterpret_cast<const i32x4_t*>(pb + k), b1 = *reinterpret_cast<const i32x4_t*>(pb + k + 16);
-    __syncthreads();
-    *reinterpret_cast<i32x4_t*>(ta + row * 80 + part) = a0;
-    *reinterpret_cast<i32x4_t*>(ta + row * 80 + part + 16) = a1;
-    *reinterpret_cast<i32x4_t*>(tb + row * 80 + part) = b0;
-    *reinterpret_cast<i32x4_t*>(tb + row * 80 + part + 16) = b1;
-    __syncthreads();
+__device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) { return (T)((float)acc * sa * sb + bias); }
+
+// ------------------------------------------------------------------------------------------------------- few rows (m <= 32)
+// The weight is read once, straight from memory into matrix operands (a lane's 16 bytes of one weight row); the rows' codes are
+// made by every workgroup for itself in LDS while the first weight loads are on their way, so one launch does it all.  NW waves
+// share a tile of 32 channels by splitting K in KS parts (joined through LDS: integer sums, any order gives the same) or work on
+// NW / KS tiles.  Bound by the latency of load - maximum - codes - product for small weights, by HBM for large ones.
+struct FewArgs {
+  const void* x;                      // rows of X, or codes with scales sa
+  Int8Args g;
+  int64_t ldx;
+  int cols;
+};
+
+template <typename X, typename Y, int NW, int KS>
+__global__ __launch_bounds__(NW * 64) void int8_few_rows_kernel(FewArgs f) {
+  constexpr int G = NW / KS, AHEAD = 6;
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  const Int8Args& g = f.g;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fi = lane & 31, fh = lane >> 5;
+  const int m = (int)g.m, pitch = g.k + 16;
+  float* scales = reinterpret_cast<float*>(smem + (size_t)m * pitch);           // (pitch is a multiple of 16)
+  int* part = reinterpret_cast<int*>(scales + 32);                              // [NW][m <= 32 rows: 16 x 64], used for KS > 1
+  const int slice = wave % KS, steps = g.k / 32;
+  const int lo = steps * slice / KS, hi = steps * (slice + 1) / KS;
+  const int64_t tiles = (g.n + 31) / 32, stride = (int64_t)gridDim.x * G;
+  int64_t tile = (int64_t)blockIdx.x * G + wave / KS;
+  auto row_of = [&](int64_t t) {
+    int64_t r = t * 32 + fi;
+    r = r < g.n ? r : g.n - 1;
+    return g.b + r * g.ldb + fh * 16;
+  };
+  i32x4_t first[AHEAD];
+  {
+    const int8_t* pb = row_of(tile < tiles ? tile : tiles - 1);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      i32x4_t af[2], bf[2];
+    for (int i = 0; i < AHEAD; ++i) first[i] = *reinterpret_cast<const i32x4_t*>(pb + (lo + i < steps ? lo + i : steps - 1) * 32);
+  }
+  // ---- codes of the rows
+  if constexpr (std::is_same_v<X, int8_t>) {
+    for (int i = threadIdx.x; i < m * (g.k / 16); i += NW * 64) {
+      const int r = i / (g.k / 16), c = i % (g.k / 16);
+      *reinterpret_cast<i32x4_t*>(smem + r * pitch + c * 16) = *reinterpret_cast<const i32x4_t*>(reinterpret_cast<const int8_t*>(f.x) + r * f.ldx + c * 16);
+    }
+    if (threadIdx.x < m) scales[threadIdx.x] = g.sa[threadIdx.x];
+  } else {
+    for (int r = wave; r < m; r += NW) {
+      const X* row = reinterpret_cast<const X*>(f.x) + r * f.ldx;
+      constexpr int HELD = 4;                      // a row of up to 64 * 8 * HELD elements is read once
+      float v[HELD][8], top = 0.f;
+      bool bad = false;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        af[i] = *reinterpret_cast<const i32x4_t*>(ta + (wm * 64 + i * 32 + fi) * 80 + ks * 32 + fh * 16);
-        bf[i] = *reinterpret_cast<const i32x4_t*>(tb + (wn * 64 + i * 32 + fi) * 80 + ks * 32 + fh * 16);
+      for (int p = 0; p < HELD; ++p)
+        if (p * 512 < f.cols) q8_load8(row, p * 512 + lane * 8, f.cols, v[p]);
+#pragma unroll
+      for (int p = 0; p < HELD; ++p)
+        if (p * 512 < f.cols) top = q8_top8(v[p], top, bad);
+      float w[8];
+      for (int k = HELD * 512 + lane * 8; k < f.cols; k += 512) {
+        q8_load8(row, k, f.cols, w);
+        top = q8_top8(w, top, bad);
       }
+      top = q8_max_group(bad ? __builtin_huge_valf() : top, 64);
+      const bool finite = top < __builtin_huge_valf();
+      const float s = finite ? q8_scale(top) : 0.f, inv = s > 0.f ? 1.f / s : 0.f;
+      uint2* out = reinterpret_cast<uint2*>(smem + r * pitch);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[i], bf[j], acc[i][j], 0, 0, 0);
+      for (int p = 0; p < HELD; ++p) {
+        const int k = p * 512 + lane * 8;
+        if (k < g.k) out[k / 8] = s > 0.f ? q8_pack8(v[p], s, inv) : make_uint2(0u, 0u);
+      }
+      for (int k = HELD * 512 + lane * 8; k < g.k; k += 512) {
+        q8_load8(row, k, f.cols, w);
+        out[k / 8] = s > 0.f ? q8_pack8(w, s, inv) : make_uint2(0u, 0u);
+      }
+      if (lane == 0) scales[r] = finite ? s : __builtin_nanf("");
     }
   }
-  T* y = reinterpret_cast<T*>(g.y);
+  __syncthreads();
+  Y* y = reinterpret_cast<Y*>(g.y);
+  const int8_t* pa = smem + (fi < m ? fi : m - 1) * pitch + fh * 16;
+  auto store = [&](int64_t t, int r, int sum, float sb, float bias) {
+    const int row = (r & 3) + 8 * (r >> 2) + 4 * fh;
+    const int64_t col = t * 32 + fi;
+    if (row < m && col < g.n) y[row * g.ldy + col] = q8_out<Y>(sum, scales[row], sb, bias);
+  };
+  bool held = true;
+  for (int64_t base = (int64_t)blockIdx.x * G; base < tiles; base += stride, tile += stride) {      // uniform over the workgroup
+    const bool live = tile < tiles;
+    const int8_t* pb = row_of(live ? tile : tiles - 1);
+    const int64_t col = tile * 32 + fi < g.n ? tile * 32 + fi : g.n - 1;
+    const float sb = g.sb[col], bias = g.bias ? g.bias[col] : 0.f;
+    i32x16_t acc = {};
+    for (int ks = lo; ks < hi; ks += AHEAD) {
+      i32x4_t bf[AHEAD];
+      if (held) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t col = n0 + wn * 64 + j * 32 + fi;
-    const bool in = col < g.n;
-    const float sb = in ? g.sb[col] : 0.f, bias = in && g.bias ? g.bias[col] : 0.f;
+        for (int i = 0; i < AHEAD; ++i) bf[i] = first[i];
+        held = false;
+      } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < AHEAD; ++i) bf[i] = *reinterpret_cast<const i32x4_t*>(pb + (ks + i < steps ? ks + i : steps - 1) * 32);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (ks + i < hi) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4_t*>(pa + (ks + i) * 32), bf[i], acc, 0, 0, 0);
+    }
+    if constexpr (KS == 1) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (live) store(tile, r, acc[r], sb, bias);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if ((r & 3) + 8 * (r >> 2) < m) part[(wave * 16 + r) * 64 + lane] = acc[r];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 16 / KS; ++i) {
+        const int r = slice * (16 / KS) + i;
+        if ((r & 3) + 8 * (r >> 2) < m) {
+          int sum = 0;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) sum += part[((wave - slice + k) * 16 + r) * 64 + lane];
+          if (live) store(tile, r, sum, sb, bias);
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ tiles of rows
+typedef __attribute__((address_space(3))) char q8_lds_char;
+
+__device__ __forceinline__ i32x4_t q8_srd(const void* base, int64_t bytes) {
+  const uint64_t b = (uint64_t)base;
+  i32x4_t r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(bytes < 0x7fffffff ? (bytes > 0 ? bytes : 0) : 0x7fffffff));
+  r[3] = 0x00020000;
+  return r;
+}
+// 64 lanes x 16 bytes from descriptor + voff + soff into LDS at lds_addr + 16 * lane; zeros from the descriptor's end on.  The
+// compiler does not see it: the kernel waits with its own counts.
+__device__ __forceinline__ void q8_dma(unsigned voff, i32x4_t srd, unsigned soff, unsigned lds_addr) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(voff), "s"(srd), "s"(soff), "s"(lds_addr) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void q8_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void q8_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename T>
+struct Q8Pair {
+  typedef T type __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+};
+
+// TM x TN outputs per workgroup of 4 waves (2 x 2), operands through LDS in steps of 128 bytes of K, NS steps in flight.  LDS image:
+// rows of 128 bytes, chunk of 16 bytes ^= row & 7 (applied to the source address of the LDS-DMA, undone by the fragment reads:
+// eight rows of one chunk fall into eight different bank groups).  Weight row 2 i + j of a wave's 64-column block lies at image row
+// 32 j + i: a lane then owns two neighbouring columns and stores them together.
+template <typename Y, int TM, int TN, int NS>
+__global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n) {
+  constexpr int STEP = 128, STAGE = (TM + TN) * STEP, QA = TM / 32, QB = TN / 32;      // DMA instructions per wave and operand
+  constexpr int WM = TM / 2, WN = TN / 2, MI = WM / 32, NJ = WN / 64;
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  const unsigned lds0 = (unsigned)(uintptr_t)(q8_lds_char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  const int fi = lane & 31, fh = lane >> 5;
+  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * TM, n0 = (int64_t)(blockIdx.x % tiles_n) * TN;
+  const int64_t rows_a = g.m - m0 < TM ? g.m - m0 : TM, rows_b = g.n - n0 < TN ? g.n - n0 : TN;
+  const i32x4_t sa = q8_srd(g.a + m0 * g.lda, rows_a * g.lda), sb = q8_srd(g.b + n0 * g.ldb, rows_b * g.ldb);
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  unsigned offa[QA], offb[QB];
+#pragma unroll
+  for (int q = 0; q < QA; ++q) offa[q] = (unsigned)((q * 4 + wave) * 8 + (lane >> 3)) * (unsigned)g.lda + chunk * 16;
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const int p = (q * 4 + wave) * 8 + (lane >> 3);
+    offb[q] = (unsigned)((p & ~63) + 2 * (p & 31) + ((p >> 5) & 1)) * (unsigned)g.ldb + chunk * 16;
+  }
+  const int steps = (g.k + STEP - 1) / STEP;
+  auto request = [&](int t) {                       // (a step past the end asks for nothing: zeros)
+    const unsigned at = lds0 + (t % NS) * STAGE, soff = t * STEP;
+    const bool in = t * STEP + chunk * 16 < g.k;
+#pragma unroll
+    for (int q = 0; q < QA; ++q) q8_dma(in ? offa[q] : 0x80000000u, sa, soff, __builtin_amdgcn_readfirstlane(at + (q * 4 + wave) * 1024));
+#pragma unroll
+    for (int q = 0; q < QB; ++q) q8_dma(in ? offb[q] : 0x80000000u, sb, soff, __builtin_amdgcn_readfirstlane(at + TM * STEP + (q * 4 + wave) * 1024));
+  };
+  i32x16_t acc[MI][NJ][2] = {};
+#pragma unroll
+  for (int t = 0; t < NS; ++t) request(t);
+  int foff[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) foff[ks] = fi * STEP + (((2 * ks + fh) ^ (fi & 7)) << 4);
+  for (int t = 0; t < steps; ++t) {
+    q8_wait<(NS - 1) * (QA + QB)>();                // step t has landed; the later ones stay in flight
+    q8_barrier();
+    const int8_t* st = smem + (t % NS) * STAGE;
+    const int8_t *pa = st + wm * WM * STEP, *pb = st + TM * STEP + wn * WN * STEP;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      i32x4_t af[MI], bf[NJ][2];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(pa + i * 32 * STEP + foff[ks]);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bf[j][h] = *reinterpret_cast<const i32x4_t*>(pb + (j * 64 + h * 32) * STEP + foff[ks]);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) acc[i][j][h] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[i], bf[j][h], acc[i][j][h], 0, 0, 0);
+    }
+    q8_barrier();                                   // everybody has read this stage
+    request(t + NS);
+  }
+  q8_wait<0>();
+  Y* y = reinterpret_cast<Y*>(g.y);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int64_t col = n0 + wn * WN + j * 64 + 2 * fi;
+    const bool two = col + 1 < g.n;
+    if (col >= g.n) continue;
+    const float s0 = g.sb[col], s1 = two ? g.sb[col + 1] : 0.f;
+    const float b0 = g.bias ? g.bias[col] : 0.f, b1 = g.bias && two ? g.bias[col + 1] : 0.f;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int64_t rw = m0 + wm * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh;
-        if (in && rw < g.m) y[rw * g.ldy + col] = (T)((float)acc[i][j][r] * g.sa[rw] * sb + bias);
+        const int64_t row = m0 + wm * WM + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh;
+        if (row >= g.m) continue;
+        const float s = g.sa[row];
+        const Y y0 = q8_out<Y>(acc[i][j][0][r], s, s0, b0), y1 = q8_out<Y>(acc[i][j][1][r], s, s1, b1);
+        if (two) {
+          typename Q8Pair<Y>::type v;
+          v[0] = y0;
+          v[1] = y1;
+          *reinterpret_cast<typename Q8Pair<Y>::type*>(y + row * g.ldy + col) = v;
+        } else {
+          y[row * g.ldy + col] = y0;
+        }
       }
   }
 }
@@ -124,34 +391,118 @@ int q8_by_type(int dtype, F f) {
 }
 
 constexpr int64_t Q8_GRID = (1 << 24) - 1;
+constexpr int64_t Q8_FEW = 32;                     // rows of the kernel that makes their codes itself
+constexpr int64_t Q8_FEW_LDS = 64 * 1024;          // ... where these fit
+
+int64_t q8_padded(int64_t k) { return (k + 63) / 64 * 64; }
+bool q8_few(int64_t m, int64_t k) { return m <= Q8_FEW && m * (q8_padded(k) + 16) <= Q8_FEW_LDS; }
+
+// a launch that may need more than 64 KB of LDS
+template <typename K, typename... A>
+int q8_launch(K kernel, dim3 grid, int threads, size_t lds, void* stream, A... args) {
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, (hipStream_t)stream, args...);
+  return (int)hipGetLastError();
+}
+
+template <typename X, typename Y>
+int q8_few_rows(const FewArgs& f, void* stream) {
+  const int64_t tiles = (f.g.n + 31) / 32;
+  const size_t base = (size_t)f.g.m * (f.g.k + 16) + 32 * 4;
+  auto go = [&](auto nw, auto ks) {
+    constexpr int NW = decltype(nw)::value, KS = decltype(ks)::value;
+    const int64_t groups = (tiles + NW / KS - 1) / (NW / KS);
+    return q8_launch(int8_few_rows_kernel<X, Y, NW, KS>, dim3((unsigned)std::min<int64_t>(groups, 2048)), NW * 64,
+                     base + (KS > 1 ? (size_t)NW * 4096 : 0), stream, f);
+  };
+  // 32 channels to a workgroup while that leaves compute units idle, and more waves along K the fewer there are
+  if (tiles <= 64 && f.g.k >= 512) return go(std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+  if (tiles <= 1024 && f.g.k >= 128) return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+  return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+}
+
+template <typename Y>
+int q8_tiles(const Int8Args& g, void* stream) {
+  auto go = [&](auto tm, auto tn, auto ns) -> int {
+    constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, NS = decltype(ns)::value;
+    const int64_t a = (g.m + TM - 1) / TM, b = (g.n + TN - 1) / TN;
+    if (b > Q8_GRID || a > Q8_GRID / b) return TN_E_UNSUPPORTED;
+    return q8_launch(int8_tile_kernel<Y, TM, TN, NS>, dim3((unsigned)(a * b)), 256, (size_t)NS * (TM + TN) * 128, stream, g, (int)b);
+  };
+  return go(std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
+}
+
+bool q8_operands_ok(int64_t m, int64_t n, int64_t k, const void* b, const float* b_scales, int64_t ldb, const void* y, int64_t ldy) {
+  if (m < 0 || n < 0 || k < 1 || ldb % 64 || ldb < k || ldy < n) return false;
+  return !m || !n || (b && b_scales && y && (uintptr_t)b % 16 == 0);
+}
 
 }  // namespace
 
 extern "C" int tn_int8_quantize_rows(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx, void* codes, int64_t ld_codes,
                                      float* scales, void* stream) {
-  if (rows < 0 || cols < 1 || ldx < 0 || ld_codes % 64 || ld_codes < cols || (rows > 0 && (!x || !codes || !scales))) return TN_E_BADARG;
+  if (rows < 0 || cols < 1 || ldx < 0 || ld_codes % 64 || ld_codes < cols || (rows > 0 && (!x || !codes || !scales || (uintptr_t)codes % 16))) return TN_E_BADARG;
   if (cols > TN_INT8_MAX_K || dtype < TN_DTYPE_F32 || dtype > TN_DTYPE_F16) return TN_E_UNSUPPORTED;
   if (!rows) return 0;
   return q8_by_type(dtype, [&](auto* kind) -> int {
     using T = std::remove_pointer_t<decltype(kind)>;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_rows_kernel<T>), dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 20)), dim3(256), 0,
-                       (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx, (int8_t*)codes, ld_codes, scales);
-    return (int)hipGetLastError();
+    auto go = [&](auto group, auto passes) {
+      constexpr int GROUP = decltype(group)::value, PASSES = decltype(passes)::value;
+      const int64_t per = 4 * (64 / GROUP);
+      return q8_launch(quantize_rows_kernel<T, GROUP, PASSES>, dim3((unsigned)std::min<int64_t>((rows + per - 1) / per, 1 << 20)), 256, 0, stream, (const T*)x,
+                       rows, (int)cols, ldx, (int8_t*)codes, ld_codes, (int)q8_padded(cols), scales);
+    };
+    using std::integral_constant;
+    // as few lanes as hold a row in one pass, so that short rows leave none idle; then more passes of a whole wave
+    if (cols <= 64) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    if (cols <= 128) return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (cols <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    if (cols <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (cols <= 1024) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (cols <= 1536) return go(integral_constant<int, 64>{}, integral_constant<int, 3>{});
+    if (cols <= 2048) return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if (cols <= 4096) return go(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+    return go(integral_constant<int, 64>{}, integral_constant<int, 0>{});
   });
 }
 
 extern "C" int tn_int8_matmul(const void* a, const float* a_scales, int64_t lda, const void* b, const float* b_scales, int64_t ldb,
                               const float* bias, void* y, int32_t y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, void* stream) {
-  if (m < 0 || n < 0 || k < 1 || lda % 64 || ldb % 64 || lda < k || ldb < k || ldy < n) return TN_E_BADARG;
-  if (m > 0 && n > 0 && (!a || !a_scales || !b || !b_scales || !y || ((uintptr_t)a | (uintptr_t)b) % 16)) return TN_E_BADARG;
+  if (!q8_operands_ok(m, n, k, b, b_scales, ldb, y, ldy) || lda % 64 || lda < k || (m > 0 && n > 0 && (!a || !a_scales || (uintptr_t)a % 16))) return TN_E_BADARG;
   if (k > TN_INT8_MAX_K || y_dtype < TN_DTYPE_F32 || y_dtype > TN_DTYPE_F16) return TN_E_UNSUPPORTED;
   if (!m || !n) return 0;
-  const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128;
-  if (tn > Q8_GRID || tm > Q8_GRID / tn) return TN_E_UNSUPPORTED;
-  const Int8Args g = {(const int8_t*)a, (const int8_t*)b, a_scales, b_scales, bias, y, lda, ldb, ldy, m, n, (int)((k + 63) / 64 * 64)};
+  const Int8Args g = {(const int8_t*)a, (const int8_t*)b, a_scales, b_scales, bias, y, lda, ldb, ldy, m, n, (int)q8_padded(k)};
   return q8_by_type(y_dtype, [&](auto* kind) -> int {
-    using T = std::remove_pointer_t<decltype(kind)>;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(int8_matmul_kernel<T>), dim3((unsigned)(tm * tn)), dim3(256), 0, (hipStream_t)stream, g, (int)tn);
-    return (int)hipGetLastError();
+    using Y = std::remove_pointer_t<decltype(kind)>;
+    if (q8_few(m, k)) return q8_few_rows<int8_t, Y>(FewArgs{a, g, lda, (int)k}, stream);
+    return q8_tiles<Y>(g, stream);
   });
+}
+
+extern "C" int64_t tn_int8_linear_workspace(int64_t m, int64_t k) {
+  if (m < 0 || k < 1 || k > TN_INT8_MAX_K) return TN_E_BADARG;
+  return q8_few(m, k) ? 0 : m * q8_padded(k) + (m + 3) / 4 * 16;
+}
+
+extern "C" int tn_int8_linear(const void* x, int32_t x_dtype, int64_t ldx, const void* b, const float* b_scales, int64_t ldb, const float* bias,
+                              void* y, int32_t y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  if (!q8_operands_ok(m, n, k, b, b_scales, ldb, y, ldy) || ldx < 0 || (m > 0 && n > 0 && !x)) return TN_E_BADARG;
+  if (k > TN_INT8_MAX_K || y_dtype < TN_DTYPE_F32 || y_dtype > TN_DTYPE_F16 || x_dtype < TN_DTYPE_F32 || x_dtype > TN_DTYPE_F16) return TN_E_UNSUPPORTED;
+  if (!m || !n) return 0;
+  if (q8_few(m, k)) {
+    const Int8Args g = {nullptr, (const int8_t*)b, nullptr, b_scales, bias, y, 0, ldb, ldy, m, n, (int)q8_padded(k)};
+    return q8_by_type(x_dtype, [&](auto* kx) -> int {
+      using X = std::remove_pointer_t<decltype(kx)>;
+      return q8_by_type(y_dtype, [&](auto* ky) -> int { return q8_few_rows<X, std::remove_pointer_t<decltype(ky)>>(FewArgs{x, g, ldx, (int)k}, stream); });
+    });
+  }
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < tn_int8_linear_workspace(m, k)) return TN_E_BADARG;
+  const int64_t ld = q8_padded(k);
+  float* scales = reinterpret_cast<float*>((char*)workspace + m * ld);
+  if (const int rc = tn_int8_quantize_rows(x, x_dtype, m, k, ldx, workspace, ld, scales, stream)) return rc;
+  return tn_int8_matmul(workspace, scales, ld, b, b_scales, ldb, bias, y, y_dtype, ldy, m, n, k, stream);
 }
