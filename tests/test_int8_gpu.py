@@ -216,3 +216,17 @@ def test_a_head_served_in_8_bits():
     assert torch.equal(other(x), y) and layer(x.bfloat16()).dtype == torch.bfloat16
     with pytest.raises(TypeError):
         layer.half()(x)
+
+
+@pytest.mark.parametrize("m,n,k", [(20000, 1536, 1536), (30001, 300, 640), (700, 30000, 192), (5000, 512, 512)])
+def test_every_output_of_large_products_time_after_time(m, n, k):
+    """all outputs of launches of many workgroups, several times over: waves that run ahead of others may not overwrite what these read"""
+    g = torch.Generator(device="cuda").manual_seed(20)
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, device="cuda", dtype=torch.int8) for r in (m, n))
+    sa, sb = torch.rand(m, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda")
+    want = a.float() @ b.float().t()                          # whole numbers below 2^24 on the way: exact
+    assert float(want.abs().max()) < 2 ** 23
+    want = want * sa[:, None] * sb[None, :]
+    qa, qb = Int8Rows(a, sa), Int8Rows(b, sb)
+    for _ in range(6):
+        assert torch.equal(int8_matmul(qa, qb), want)

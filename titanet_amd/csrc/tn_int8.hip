@@ -63,14 +63,28 @@ __device__ __forceinline__ float q8_top8(const float v[8], float top, bool& bad)
   for (int j = 0; j < 8; ++j) bad |= !(fabsf(v[j]) < __builtin_huge_valf());
   return top;
 }
+// Codes of eight values.  Adding 1.5 * 2^23 in one fused multiply-add leaves the nearest integer to x * inv in the sum's low byte
+// (two's complement, even half way); inv itself is off by half a step, 127 * 2^-24 of a code at most, so only where the quotient
+// comes within 2^-16 of half way the exact comparison has to decide.  5 instructions a value where the comparison alone takes 20:
+// the quantiser is bound by memory instead of by the vector pipe.
 __device__ __forceinline__ uint2 q8_pack8(const float v[8], float s, float inv) {
-  uint2 q = make_uint2(0u, 0u);
+  constexpr float MAGIC = 12582912.f;
+  float t[8], off = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    q.x |= (uint32_t)(uint8_t)q8_code(v[j], s, inv) << (8 * j);
-    q.y |= (uint32_t)(uint8_t)q8_code(v[4 + j], s, inv) << (8 * j);
+  for (int j = 0; j < 8; ++j) {
+    t[j] = fmaf(v[j], inv, MAGIC);
+    off = fmaxf(off, fabsf(fmaf(v[j], inv, -(t[j] - MAGIC))));
   }
-  return q;
+  if (off > 0.5f - 0x1p-16f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = __int_as_float(q8_code(v[j], s, inv));
+  }
+  auto four = [](const float* f) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x04000c0cu);
+    return lo | hi;
+  };
+  return make_uint2(four(t), four(t + 4));
 }
 
 // Codes and scale of every row.  A row belongs to GROUP lanes of a wave, eight elements to a lane and pass, kept in registers
@@ -285,6 +299,12 @@ __device__ __forceinline__ void q8_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// the same once this wave's LDS reads have returned: what they read may be overwritten behind it
+__device__ __forceinline__ void q8_barrier_after_reads() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  q8_barrier();
+}
+
 template <typename T>
 struct Q8Pair {
   typedef T type __attribute__((ext_vector_type(2), aligned(sizeof(T))));
@@ -305,6 +325,8 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n)
   const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * TM, n0 = (int64_t)(blockIdx.x % tiles_n) * TN;
   const int64_t rows_a = g.m - m0 < TM ? g.m - m0 : TM, rows_b = g.n - n0 < TN ? g.n - n0 : TN;
   const i32x4_t sa = q8_srd(g.a + m0 * g.lda, rows_a * g.lda), sb = q8_srd(g.b + n0 * g.ldb, rows_b * g.ldb);
+  const int tr = (int)(threadIdx.x < rows_a ? threadIdx.x : rows_a - 1), tc = (int)(threadIdx.x < rows_b ? threadIdx.x : rows_b - 1);
+  const float in_sa = g.sa[m0 + tr], in_sb = g.sb[n0 + tc], in_bias = g.bias ? g.bias[n0 + tc] : 0.f;
   const int chunk = (lane & 7) ^ (lane >> 3);
   unsigned offa[QA], offb[QB];
 #pragma unroll
@@ -315,7 +337,8 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n)
     offb[q] = (unsigned)((p & ~63) + 2 * (p & 31) + ((p >> 5) & 1)) * (unsigned)g.ldb + chunk * 16;
   }
   const int steps = (g.k + STEP - 1) / STEP;
-  auto request = [&](int t) {                       // (a step past the end asks for nothing: zeros)
+  auto request = [&](int t) {
+    if (t >= steps) return;
     const unsigned at = lds0 + (t % NS) * STAGE, soff = t * STEP;
     const bool in = t * STEP + chunk * 16 < g.k;
 #pragma unroll
@@ -330,7 +353,8 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n)
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) foff[ks] = fi * STEP + (((2 * ks + fh) ^ (fi & 7)) << 4);
   for (int t = 0; t < steps; ++t) {
-    q8_wait<(NS - 1) * (QA + QB)>();                // step t has landed; the later ones stay in flight
+    if (t + NS <= steps) q8_wait<(NS - 1) * (QA + QB)>();      // step t has landed; the later ones stay in flight
+    else q8_wait<0>();
     q8_barrier();
     const int8_t* st = smem + (t % NS) * STAGE;
     const int8_t *pa = st + wm * WM * STEP, *pb = st + TM * STEP + wn * WN * STEP;
@@ -350,36 +374,48 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) acc[i][j][h] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[i], bf[j][h], acc[i][j][h], 0, 0, 0);
     }
-    q8_barrier();                                   // everybody has read this stage
+    q8_barrier_after_reads();                       // everybody has read this stage
     request(t + NS);
   }
-  q8_wait<0>();
-  Y* y = reinterpret_cast<Y*>(g.y);
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int64_t col = n0 + wn * WN + j * 64 + 2 * fi;
-    const bool two = col + 1 < g.n;
-    if (col >= g.n) continue;
-    const float s0 = g.sb[col], s1 = two ? g.sb[col + 1] : 0.f;
-    const float b0 = g.bias ? g.bias[col] : 0.f, b1 = g.bias && two ? g.bias[col + 1] : 0.f;
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + wm * WM + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh;
-        if (row >= g.m) continue;
-        const float s = g.sa[row];
-        const Y y0 = q8_out<Y>(acc[i][j][0][r], s, s0, b0), y1 = q8_out<Y>(acc[i][j][1][r], s, s1, b1);
-        if (two) {
-          typename Q8Pair<Y>::type v;
-          v[0] = y0;
-          v[1] = y1;
-          *reinterpret_cast<typename Q8Pair<Y>::type*>(y + row * g.ldy + col) = v;
-        } else {
-          y[row * g.ldy + col] = y0;
-        }
-      }
+  // ---- epilogue: scales and bias of the tile through LDS (a load per output row would be waited for row by row)
+  float* sc = reinterpret_cast<float*>(smem);       // [TM] token scales, [TN] channel scales, [TN] bias
+  if (threadIdx.x < TM) sc[threadIdx.x] = in_sa;
+  if (threadIdx.x < TN) {
+    sc[TM + threadIdx.x] = in_sb;
+    sc[TM + TN + threadIdx.x] = in_bias;
   }
+  __syncthreads();
+  Y* y = reinterpret_cast<Y*>(g.y);
+  auto put = [&](auto whole) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int c = wn * WN + j * 64 + 2 * fi;
+      const int64_t col = n0 + c;
+      const bool two = whole || col + 1 < g.n;
+      if (!whole && col >= g.n) continue;
+      const float s0 = sc[TM + c], s1 = sc[TM + c + 1], b0 = sc[TM + TN + c], b1 = sc[TM + TN + c + 1];
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int rw = wm * WM + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh;
+          const int64_t row = m0 + rw;
+          if (!whole && row >= g.m) continue;
+          const float s = sc[rw];
+          const Y y0 = q8_out<Y>(acc[i][j][0][r], s, s0, b0), y1 = q8_out<Y>(acc[i][j][1][r], s, s1, b1);
+          if (two) {
+            typename Q8Pair<Y>::type v;
+            v[0] = y0;
+            v[1] = y1;
+            *reinterpret_cast<typename Q8Pair<Y>::type*>(y + row * g.ldy + col) = v;
+          } else {
+            y[row * g.ldy + col] = y0;
+          }
+        }
+    }
+  };
+  if (rows_a == TM && rows_b == TN) put(std::true_type{});
+  else put(std::false_type{});
 }
 
 template <typename F>
