@@ -102,6 +102,17 @@ class MetricLearningLoss(nn.Module):
             raise NotImplementedError
         return _HeadFunction.apply(inputs, self.fc.weight, self.fc.bias, self, targets)
 
+    @torch.no_grad()
+    def int8_head(self):
+        """The head's classifier as a :class:`titanet_amd.int8.Int8Linear` for serving: embeddings -> scores of every speaker (the
+        logits of reference src/losses.py:39; for the margin losses the cosines of :86-91, given L2-normalised embeddings)."""
+        if not hasattr(self, "fc"):
+            raise NotImplementedError
+        from .int8 import Int8Linear
+        if self.fc.bias is not None:
+            return Int8Linear.from_linear(self.fc)
+        return Int8Linear(nn.functional.normalize(self.fc.weight, dim=1))
+
     def native_config(self):
         """(loss_type, has_scale, scale, m1, m2, m3, eps) for tn_config."""
         return (self.tn_loss_type, 1, 1.0, 1.0, 0.0, 0.0, 1e-6)

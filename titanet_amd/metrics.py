@@ -72,13 +72,34 @@ def get_test_metrics(scores, labels, mindcf_p_target=1e-2, mindcf_c_fa=1, mindcf
 
 
 @torch.no_grad()
-def verification_test(model, spectrograms, speakers, mindcf_p_target=1e-2, mindcf_c_fa=1, mindcf_c_miss=1, batch_size=64):
+def cosine_scores(embeddings, enrolled=None, bits=32):
+    """Cosine similarity of every row of ``embeddings`` [m, E] with every row of ``enrolled`` [n, E] (default: the embeddings
+    themselves), as float32 [m, n] on their device (the scores of reference src/learn.py:441-447, all pairs at once).
+
+    ``bits=8`` multiplies in 8-bit integers (:mod:`titanet_amd.int8`): a quarter of the memory for the enrolled side, which can be
+    handed over quantised once — ``quantize_rows`` of L2-normalised embeddings."""
+    if bits not in (8, 32):
+        raise ValueError(f"bits must be 8 or 32, got {bits!r}")
+
+    def unit(e):
+        return e / e.norm(dim=1, keepdim=True).clamp(min=1e-8)       # F.cosine_similarity eps
+    e = unit(embeddings)
+    if bits == 32:
+        return e @ (e if enrolled is None else unit(enrolled)).t()
+    from .int8 import Int8Rows, int8_matmul, quantize_rows
+    rows = quantize_rows(e) if enrolled is None else enrolled if isinstance(enrolled, Int8Rows) else quantize_rows(unit(enrolled))
+    return int8_matmul(rows if enrolled is None else e, rows, out_dtype=torch.float32)
+
+
+@torch.no_grad()
+def verification_test(model, spectrograms, speakers, mindcf_p_target=1e-2, mindcf_c_fa=1, mindcf_c_miss=1, batch_size=64, score_bits=32):
     """``learn.test`` (reference src/learn.py:409-459) without its 200x redundant forward passes:
     every utterance is embedded ONCE, ``batch_size`` utterances per forward: the batch is zero-padded to its longest
     utterance and run with the padding mask (``lengths=``), which makes every row equal to that utterance embedded on
     its own (eval mode: running statistics; tests/test_mask_gpu.py) — what the reference computes with B = 1 per pair.
     Then all ordered pairs including self-pairs (itertools.product(indices, repeat=2), src/datasets.py:171-183) are scored
     with the cosine similarity of the L2-normalised embeddings.
+    ``score_bits=8``: the pairs are scored in 8-bit integers (:func:`cosine_scores`).
     spectrograms: list of [n_mels, T_i] or [1, n_mels, T_i] tensors; speakers: list of ids."""
     was_training = model.training
     model.eval()
@@ -109,9 +130,7 @@ def verification_test(model, spectrograms, speakers, mindcf_p_target=1e-2, mindc
                 emb_of[i] = e[k:k + 1]
     embs = emb_of
     model.train(was_training)
-    e = torch.cat(embs, dim=0)
-    e = e / e.norm(dim=1, keepdim=True).clamp(min=1e-8)       # F.cosine_similarity eps
-    sim = (e @ e.t()).cpu().numpy()
+    sim = cosine_scores(torch.cat(embs, dim=0), bits=score_bits).cpu().numpy()
     n = len(spectrograms)
     pairs = list(itertools.product(range(n), repeat=2))
     scores = np.array([sim[i, j] for i, j in pairs])

@@ -69,7 +69,7 @@ def init_distributed(backend="nccl", same_device=False):
 
 
 def run(params, steps=None, n_classes=251, data=None, device="cuda", precision="fp32", log_every=10, resume=None,
-        use_graph=False, rank=0, world=1, grad_groups=2):
+        use_graph=False, rank=0, world=1, grad_groups=2, optimizer="adam", state_bits=32, max_grad_norm=None):
     torch.manual_seed(params.generic.seed)            # same initial weights on every rank (rank 0's are broadcast anyway)
     loss_name = params.training.loss
     loss_kw = dict(getattr(params.loss, loss_name).entries) if hasattr(params.loss, loss_name) else {}
@@ -80,7 +80,8 @@ def run(params, steps=None, n_classes=251, data=None, device="cuda", precision="
                                 loss_function=loss_function, dropout=params.titanet.dropout, device=device, precision=precision)
     model.train()
     opt = params.training.optimizer
-    trainer = Trainer(model, lr=opt.start_lr, weight_decay=opt.weight_decay, use_graph=use_graph, n_buckets=grad_groups)
+    trainer = Trainer(model, lr=opt.start_lr, weight_decay=opt.weight_decay, use_graph=use_graph, n_buckets=grad_groups,
+                      optimizer=optimizer, state_bits=state_bits, max_grad_norm=max_grad_norm)
     first = 1
     if resume:
         first = load_checkpoint(model, trainer, resume)[0] + 1
@@ -152,12 +153,18 @@ def main():
     ap.add_argument("--resume", default=None, help="checkpoint to resume from (reference layout, src/learn.py:188-195)")
     ap.add_argument("--backend", default="nccl", help="torch.distributed backend under torchrun (nccl == RCCL)")
     ap.add_argument("--grad-groups", type=int, default=2, help="gradient buckets of mega blocks (overlapped all-reduce)")
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "adamw"], help="adam: the reference's; adamw: decoupled weight decay")
+    ap.add_argument("--state-bits", type=int, default=32, choices=[8, 32], help="bits of adamw's moments")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="adamw: clip the gradient to this norm")
     args = ap.parse_args()
+    if args.optimizer == "adam" and (args.state_bits != 32 or args.max_grad_norm is not None):
+        ap.error("--state-bits and --max-grad-norm belong to --optimizer adamw")
     with open(args.params) as fh:
         params = Struct(**yaml.load(fh, Loader=yaml.SafeLoader))
     rank, world, device = init_distributed(args.backend)
     model, trainer, _ = run(params, steps=args.steps, precision=args.precision, resume=args.resume, device=device, rank=rank,
-                            world=world, grad_groups=args.grad_groups)
+                            world=world, grad_groups=args.grad_groups, optimizer=args.optimizer, state_bits=args.state_bits,
+                            max_grad_norm=args.max_grad_norm)
     if args.checkpoint and rank == 0:          # replicas are identical: rank 0 writes (its BatchNorm running statistics, as DDP)
         opt = params.training.optimizer
         epoch = args.steps or params.training.epochs

@@ -121,7 +121,11 @@ class Trainer:
     """``step(spectrograms, speakers)`` == one iteration of reference src/learn.py:88-135."""
 
     def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, n_buckets=2, group=None,
-                 use_graph=False, graph_warmup=2, max_steps_in_flight=0):
+                 use_graph=False, graph_warmup=2, max_steps_in_flight=0, optimizer="adam", state_bits=32, max_grad_norm=None):
+        if optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer must be 'adam' or 'adamw', got {optimizer!r}")
+        if optimizer == "adam" and (state_bits != 32 or max_grad_norm is not None):
+            raise ValueError("state_bits and max_grad_norm belong to optimizer='adamw'")
         self.model = model
         # A step is 400-600 kernel launches and the host enqueues one in ~1.2 ms: left alone it runs a few steps ahead of the
         # GPU until the HIP runtime's own back-pressure blocks it (a sleeping wait: harmless, the GPU stays fed).  Optional
@@ -137,8 +141,17 @@ class Trainer:
         self.graph_warmup = graph_warmup
         self._graphs = {}          # (B, T) -> dict(graph, x, y, out, eager_steps)
         flat = model.flat_parameters()
-        self.exp_avg = torch.zeros_like(flat)
-        self.exp_avg_sq = torch.zeros_like(flat)
+        self.adamw, self._lr_dev = None, None
+        if optimizer == "adamw":
+            # decoupled decay, optional 8-bit moments and clipping by the norm of the (reduced) gradient: titanet_amd.optim over
+            # the flat buffer as ONE tensor
+            from .optim import AdamW
+            self._flat = flat.detach()
+            self.adamw = AdamW([self._flat], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                               max_grad_norm=max_grad_norm, grad_mult=1.0 / self.reducer.world)
+        else:
+            self.exp_avg = torch.zeros_like(flat)
+            self.exp_avg_sq = torch.zeros_like(flat)
         if self.reducer.world > 1:
             # replicas start identical (rank 0's weights), as DDP does
             dist.broadcast(flat, src=0, group=group)
@@ -163,10 +176,28 @@ class Trainer:
         self._last_plan = plan
         return emb, preds, loss
 
+    def _adamw_step(self, lr):
+        """the trainer's hyper-parameters and the model's present buffers, then one step"""
+        m = self.model
+        if self._flat.data_ptr() != m.flat_parameters().data_ptr():
+            self._flat.data = m.flat_parameters()
+        if self._flat.grad is None or self._flat.grad.data_ptr() != m.flat_gradients().data_ptr():
+            self._flat.grad = m.flat_gradients()
+        self.adamw.param_groups[0].update(lr=lr, betas=tuple(self.betas), eps=self.eps, weight_decay=self.weight_decay)
+        self.adamw.step()
+
+    @property
+    def last_grad_norm(self):
+        """the gradient's norm before clipping (0-dim device tensor; AdamW with ``max_grad_norm``, else None)"""
+        return self.adamw.last_grad_norm if self.adamw is not None else None
+
     def optimizer_step(self):
         m = self.model
         flat, grads = m.flat_parameters(), m.flat_gradients()
         self.step_count += 1
+        if self.adamw is not None:
+            self._adamw_step(float(self.lr))
+            return
         stream = torch.cuda.current_stream(flat.device).cuda_stream
         vp = C.c_void_p
         check(m._lib.tn_adam_step(vp(flat.data_ptr()), vp(grads.data_ptr()), vp(self.exp_avg.data_ptr()),
@@ -224,30 +255,41 @@ class Trainer:
         .load_state_dict(...)`` accepts it, and :meth:`load_optimizer_state_dict` accepts an Adam state_dict."""
         sl = self._param_slices()
         state = {}
+        if self.adamw is not None:      # (8-bit moments as the float32 values of their codes, from which the same codes come back)
+            exp_avg, exp_avg_sq = self.adamw.moments()
+            done = self.adamw.state_dict()["state"].get(0)
+            steps = float(done["step"]) if done else 0.0
+        else:
+            exp_avg, exp_avg_sq, steps = self.exp_avg, self.exp_avg_sq, float(self.step_count)
         for i, (off, numel, shape) in enumerate(sl):
-            state[i] = {"step": torch.tensor(float(self.step_count)),
-                        "exp_avg": self.exp_avg[off:off + numel].view(shape).clone(),
-                        "exp_avg_sq": self.exp_avg_sq[off:off + numel].view(shape).clone()}
+            state[i] = {"step": torch.tensor(steps),
+                        "exp_avg": exp_avg[off:off + numel].view(shape).clone(),
+                        "exp_avg_sq": exp_avg_sq[off:off + numel].view(shape).clone()}
         group = {"lr": self.lr, "betas": tuple(self.betas), "eps": self.eps, "weight_decay": self.weight_decay, "amsgrad": False,
                  "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
-                 "decoupled_weight_decay": False, "params": list(range(len(sl)))}
+                 "decoupled_weight_decay": self.adamw is not None, "params": list(range(len(sl)))}
         return {"state": state, "param_groups": [group]}
 
     def load_optimizer_state_dict(self, sd):
         sl = self._param_slices()
         g = sd["param_groups"][0]
         self.lr, self.betas, self.eps, self.weight_decay = g["lr"], tuple(g["betas"]), g["eps"], g["weight_decay"]
-        self.exp_avg.zero_()
-        self.exp_avg_sq.zero_()
+        if self.adamw is not None:
+            size = self.adamw.moments()[0].numel()
+            exp_avg, exp_avg_sq = (torch.zeros(size, dtype=torch.float32, device=self.model.flat_parameters().device) for _ in range(2))
+        else:
+            exp_avg, exp_avg_sq = self.exp_avg.zero_(), self.exp_avg_sq.zero_()
         step = 0
         for i, (off, numel, shape) in enumerate(sl):
             st = sd["state"].get(i)
             if st is None:
                 continue
-            self.exp_avg[off:off + numel].view(shape).copy_(st["exp_avg"])
-            self.exp_avg_sq[off:off + numel].view(shape).copy_(st["exp_avg_sq"])
+            exp_avg[off:off + numel].view(shape).copy_(st["exp_avg"])
+            exp_avg_sq[off:off + numel].view(shape).copy_(st["exp_avg_sq"])
             step = max(step, int(float(st["step"])))
         self.step_count = step
+        if self.adamw is not None:
+            self.adamw.load_moments(exp_avg, exp_avg_sq, step=step)
         for st in self._graphs.values():      # captured graphs hold no optimizer state, but restart their warm-up
             st["graph"], st["eager"] = None, 0
 
@@ -261,6 +303,9 @@ class Trainer:
         check(m._lib.tn_plan_step_tick(plan.handle, vp(stream)), "tn_plan_step_tick")
         emb, preds, loss, plan = m._native_forward(x, y, fixed_seed=True)
         check(m._lib.tn_backward(plan.handle, C.c_float(1.0), vp(0), vp(0), vp(0), vp(stream)), "tn_backward")
+        if self.adamw is not None:
+            self._adamw_step(self._lr_dev)          # (a device word, like the plan's below)
+            return emb, preds, loss, plan
         flat, grads = m.flat_parameters(), m.flat_gradients()
         # lr < 0: read the plan's device lr word (written by _sync_device_state before every step, so a scheduler that
         # assigns trainer.lr keeps working under graph replay); betas / eps / weight decay are captured by value — changing
@@ -277,6 +322,11 @@ class Trainer:
         m = self.model
         stream = torch.cuda.current_stream(device).cuda_stream
         check(m._lib.tn_plan_step_set(plan.handle, self.step_count - 1, C.c_void_p(stream)), "tn_plan_step_set")
+        if self.adamw is not None:
+            if self._lr_dev is None:
+                self._lr_dev = torch.empty((), dtype=torch.float32, device=device)
+            self._lr_dev.fill_(float(self.lr))
+            return
         check(m._lib.tn_plan_set_lr(plan.handle, C.c_float(float(self.lr)), C.c_void_p(stream)), "tn_plan_set_lr")
 
     def _graph_step(self, spectrograms, speakers):
@@ -288,7 +338,7 @@ class Trainer:
         st["x"].copy_(spectrograms)
         st["y"].copy_(speakers)
         self.step_count += 1
-        hp = (tuple(self.betas), self.eps, self.weight_decay)
+        hp = (tuple(self.betas), self.eps, self.weight_decay, self.adamw.max_grad_norm if self.adamw is not None else None)
         if st["graph"] is not None and (self.model._plans.get(st["plan"].key) is not st["plan"] or st["hp"] != hp):
             st["graph"], st["eager"] = None, 0          # plan evicted from the model's cache / captured hyper-parameters changed
         plan = self.model._get_plan(st["x"].shape[0], st["x"].shape[2])
