@@ -203,14 +203,33 @@ int tn_plan_set_lr(tn_plan* p, float lr, void* stream);
  * on (the rest of its last block is padding and holds zeros).  state_bits 32: float moments.  state_bits 8: one byte per element and one float scale
  * per block,  exp_avg = sign (c / 127)^2 scale,  exp_avg_sq = (c / 255)^4 scale, nearest code, the lower one half way, and no
  * exp_avg_sq above 0 gets code 0; a block with a NaN or an infinity gets the scale NaN.
- * A step is: tn_grad_sumsq for each list of gradients and tn_grad_norm_finish (where the norm clips), tn_adamw_tick once for
- * each set of hyper-parameters, tn_adamw_apply for each list of tensors of one type.  Everything that changes from step to step
- * (counts, factor, learning rate) is in device memory: the sequence can be captured.
- * Pointer arrays are HOST arrays and are not read after the call returns.  numel may be 0. */
+ * A step is: tn_grad_sumsq for each list of gradients where the norm clips, tn_adamw_tick once for each set of
+ * hyper-parameters (the first ends the norm), tn_adamw_apply for each list of tensors of one type; or tn_adamw_step_small alone.
+ * Everything that changes from step to step (counts, factor, learning rate) is in device memory: the sequence can be captured.
+ * The structures and pointer arrays are HOST memory and are not read after the call returns.  numel may be 0. */
 #define TN_OPT_BLOCK 256
 #define TN_DTYPE_F32 0
 #define TN_DTYPE_BF16 1
 #define TN_DTYPE_F16 2
+typedef struct tn_adamw_hyper {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_dev; /* device word that replaces lr, or NULL */
+} tn_adamw_hyper;
+typedef struct tn_adamw_state { /* device memory */
+  int32_t bits;                 /* 32 or 8 */
+  int64_t blocks;               /* how many blocks of 256 the moment buffers hold */
+  void *exp_avg, *exp_avg_sq;   /* float, or int8 and uint8 */
+  float *scale1, *scale2;       /* 8 bits: [blocks] */
+  int32_t* steps;               /* by slot: tensors that have always been stepped together share one */
+  float* corr;                  /* float[4] by slot, 16-byte aligned: what the step derives from the count */
+} tn_adamw_state;
+typedef struct tn_adamw_lists { /* tensors of one type */
+  int32_t count, dtype;
+  void* const* params;
+  const void* const* grads;
+  const int64_t *numel, *first_block;
+  const int32_t* slots;
+} tn_adamw_lists;
 /* how many partial sums tn_grad_sumsq writes at most for these tensors */
 int64_t tn_grad_sumsq_partials(int32_t count, const int64_t* numel);
 /* partials: device double; *written (host): how many of them hold a sum */
@@ -219,15 +238,17 @@ int tn_grad_sumsq(int32_t count, const void* const* grads, const int64_t* numel,
 /* norm (device float, may be NULL) = |grad_mult| sqrt(sum of the partials).  ctl (device double[2], may be NULL): {grad_mult *
  * min(1, max_norm / (norm + 1e-6)), 1}, or {0, 0} where the norm is not finite: the step that reads it changes nothing then. */
 int tn_grad_norm_finish(const double* partials, int64_t count, double grad_mult, double max_norm, float* norm, double* ctl, void* stream);
-/* steps (device int32), corr (device float[4] each) are indexed by slot: tensors that have always been stepped together share
- * one.  Advances the count of each listed slot and derives its bias corrections.  lr_dev (device float) replaces lr if given. */
-int tn_adamw_tick(int32_t count, const int32_t* slots, int32_t* steps, float* corr, const double* ctl, double lr, const float* lr_dev,
-                  double beta1, double beta2, double weight_decay, void* stream);
-/* blocks: how many the moment buffers hold.  ctl NULL: gradients times grad_mult. */
-int tn_adamw_apply(int32_t count, void* const* params, const void* const* grads, const int64_t* numel, const int64_t* first_block,
-                   const int32_t* slots, int32_t dtype, int32_t state_bits, void* exp_avg, void* exp_avg_sq, float* scale1, float* scale2,
-                   int64_t blocks, const float* corr, const double* ctl, double grad_mult, double beta1, double beta2, double eps,
+/* Advances the count of each listed slot and derives its bias corrections.  With partials: does tn_grad_norm_finish first.  Without:
+ * ctl (may be NULL) is only read. */
+int tn_adamw_tick(int32_t count, const int32_t* slots, const tn_adamw_state* s, const tn_adamw_hyper* h, const double* partials,
+                  int64_t n_partials, double grad_mult, double max_norm, float* norm, double* ctl, void* stream);
+/* ctl NULL: gradients times grad_mult */
+int tn_adamw_apply(const tn_adamw_lists* l, const tn_adamw_state* s, const tn_adamw_hyper* h, double grad_mult, const double* ctl,
                    void* stream);
+/* The whole step of one set of hyper-parameters and one type in one launch; max_norm 0: no norm.  TN_E_UNSUPPORTED, with nothing
+ * launched, for lists of more than 64 blocks of 256 elements. */
+int tn_adamw_step_small(const tn_adamw_lists* l, const tn_adamw_state* s, const tn_adamw_hyper* h, int32_t n_slots, const int32_t* slots,
+                        double grad_mult, double max_norm, float* norm, void* stream);
 /* 8-bit moments -> float values [blocks * 256] and back */
 int tn_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale1, const float* scale2, float* out1, float* out2,
                       int64_t blocks, void* stream);

@@ -46,26 +46,42 @@ def test_c_entries_refuse_before_they_touch_the_device():
     n, first, slot = (C.c_int64 * 1)(256), (C.c_int64 * 1)(0), (C.c_int32 * 1)(0)
     at, written = C.c_void_p(4096), C.c_int64()
 
-    def apply(count=1, params=one, numel=n, first_block=first, slots=slot, dtype=0, bits=32, m=at, scale=at, blocks=1, b1=0.9, eps=1e-8):
-        return lib.tn_adamw_apply(count, params, one, numel, first_block, slots, dtype, bits, m, at, scale, scale, blocks, at, none, 1.0, b1, 0.999,
-                                  eps, none)
+    def call(entry, count=1, params=one, numel=n, first_block=first, slots=slot, dtype=0, bits=32, m=at, scale=at, blocks=1, b1=0.9, eps=1e-8, lr=1e-3,
+             steps=at, corr=at, wd=0.0):
+        p = lambda a: C.cast(a, C.c_void_p)  # noqa: E731
+        lists = _lib.TnAdamwLists(count, dtype, p(params), p(one), p(numel), p(first_block), p(slots))
+        state = _lib.TnAdamwState(bits, blocks, m, m, scale, scale, steps, corr)
+        hyper = _lib.TnAdamwHyper(lr, b1, 0.999, eps, wd, none)
+        if entry == "apply":
+            return lib.tn_adamw_apply(lists, state, hyper, 1.0, none, none)
+        if entry == "small":
+            return lib.tn_adamw_step_small(lists, state, hyper, 1, p(slots), 1.0, 0.0, none, none)
+        return lib.tn_adamw_tick(count, p(slots), state, hyper, none, 0, 1.0, 0.0, none, none, none)
 
     bad, unsupported = -1, -2
-    assert apply(count=0) == 0 and apply(count=-1) == bad
-    assert apply(params=(C.c_void_p * 1)(0)) == bad and apply(m=none) == bad
-    assert apply(numel=(C.c_int64 * 1)(-1)) == bad and apply(slots=(C.c_int32 * 1)(-1)) == bad
-    assert apply(numel=(C.c_int64 * 1)(257)) == bad                      # more than the moment buffers hold
-    assert apply(first_block=(C.c_int64 * 1)(1)) == bad and apply(first_block=(C.c_int64 * 1)(-1)) == bad
-    assert apply(dtype=3) == unsupported and apply(bits=16) == unsupported and apply(bits=8, scale=none) == bad
-    assert apply(b1=1.0) == bad and apply(b1=float("nan")) == bad and apply(eps=-1.0) == bad and apply(blocks=1 << 33) == unsupported
+    assert call("apply", count=0) == 0 and call("tick", count=0) == 0
+    for entry in ("apply", "small"):
+        assert call(entry, count=-1) == bad and call(entry, m=none) == bad and call(entry, corr=none) == bad
+        assert call(entry, params=(C.c_void_p * 1)(0)) == bad
+        assert call(entry, numel=(C.c_int64 * 1)(-1)) == bad and call(entry, slots=(C.c_int32 * 1)(-1)) == bad
+        assert call(entry, numel=(C.c_int64 * 1)(257)) == bad                      # more than the moment buffers hold
+        assert call(entry, numel=(C.c_int64 * 1)(2 ** 62)) == bad
+        assert call(entry, first_block=(C.c_int64 * 1)(1)) == bad and call(entry, first_block=(C.c_int64 * 1)(-1)) == bad
+        assert call(entry, dtype=3) == unsupported and call(entry, bits=16) == unsupported and call(entry, bits=8, scale=none) == bad
+        assert call(entry, blocks=1 << 33) == unsupported
+    for entry in ("apply", "small", "tick"):
+        assert call(entry, b1=1.0) == bad and call(entry, b1=float("nan")) == bad and call(entry, eps=-1.0) == bad and call(entry, lr=-1.0) == bad
+        assert call(entry, wd=float("nan")) == bad
+    assert call("small", steps=none) == bad and call("small", blocks=100, numel=(C.c_int64 * 1)(65 * 256)) == unsupported
+    assert call("tick", steps=none) == bad and call("tick", corr=none) == bad and call("tick", slots=(C.c_int32 * 1)(-1)) == bad
+    state, hyper = _lib.TnAdamwState(32, 1, at, at, none, none, at, at), _lib.TnAdamwHyper(1e-3, 0.9, 0.999, 1e-8, 0.0, none)
+    assert lib.tn_adamw_tick(1, slot, state, hyper, at, 1, 1.0, 1.0, none, none, none) == bad          # partial sums, nowhere for the factor
+    assert lib.tn_adamw_tick(1, slot, state, hyper, at, 1, 1.0, 0.0, none, at, none) == bad
     assert lib.tn_grad_sumsq_partials(-1, none) == bad and lib.tn_grad_sumsq_partials(0, none) == 0
-    assert lib.tn_grad_sumsq_partials(1, n) == 1 and lib.tn_grad_sumsq_partials(1, (C.c_int64 * 1)(16385)) == 2
+    assert lib.tn_grad_sumsq_partials(1, n) == 1 and lib.tn_grad_sumsq_partials(1, (C.c_int64 * 1)(10 ** 6)) > 1
     assert lib.tn_grad_sumsq(1, one, n, 7, at, C.byref(written), none) == unsupported
     assert lib.tn_grad_sumsq(1, (C.c_void_p * 1)(0), n, 0, at, C.byref(written), none) == bad
     assert lib.tn_grad_norm_finish(at, -1, 1.0, 1.0, at, none, none) == bad and lib.tn_grad_norm_finish(at, 1, 1.0, 0.0, at, at, none) == bad
-    assert lib.tn_adamw_tick(1, slot, at, none, none, 1e-3, none, 0.9, 0.999, 0.0, none) == bad
-    assert lib.tn_adamw_tick(1, slot, at, at, none, -1.0, none, 0.9, 0.999, 0.0, none) == bad
-    assert lib.tn_adamw_tick(1, (C.c_int32 * 1)(-1), at, at, none, 1e-3, none, 0.9, 0.999, 0.0, none) == bad
     assert lib.tn_moments_decode(none, at, at, at, at, at, 1, none) == bad and lib.tn_moments_encode(at, at, at, at, at, none, 1, none) == bad
 
 

@@ -19,7 +19,7 @@ EXPORTS = [
     "tn_profile_read", "tn_profile_sample", "tn_mel_create", "tn_mel_destroy", "tn_mel_num_frames", "tn_mel_forward", "tn_mel_forward_batch", "tn_plan_step_tick",
     "tn_plan_step_set", "tn_adam_step_plan", "tn_plan_set_lr", "tn_head_save_floats", "tn_head_forward", "tn_head_backward",
     "tn_forward_masked", "tn_forward_prepacked", "tn_plan_prolog_input", "tn_mel_forward_batch_packed", "tn_plan_set_grad_groups", "tn_plan_num_grad_buckets", "tn_plan_grad_bucket", "tn_plan_wait_grad_bucket",
-    "tn_mark_host", "tn_grad_sumsq_partials", "tn_grad_sumsq", "tn_grad_norm_finish", "tn_adamw_tick", "tn_adamw_apply", "tn_moments_decode",
+    "tn_mark_host", "tn_grad_sumsq_partials", "tn_grad_sumsq", "tn_grad_norm_finish", "tn_adamw_tick", "tn_adamw_apply", "tn_adamw_step_small", "tn_moments_decode",
     "tn_moments_encode", "tn_int8_quantize_rows", "tn_int8_matmul",
     "tn_int8_linear_workspace", "tn_int8_linear",
 ]
@@ -34,6 +34,21 @@ class TnConfig(C.Structure):
         ("dropout", C.c_float), ("scale", C.c_float), ("m1", C.c_float), ("m2", C.c_float), ("m3", C.c_float),
         ("loss_eps", C.c_float), ("simple_pool", C.c_int32),
     ]
+
+
+class TnAdamwHyper(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("lr_dev", C.c_void_p)]
+
+
+class TnAdamwState(C.Structure):
+    _fields_ = [("bits", C.c_int32), ("blocks", C.c_int64), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("scale1", C.c_void_p),
+                ("scale2", C.c_void_p), ("steps", C.c_void_p), ("corr", C.c_void_p)]
+
+
+class TnAdamwLists(C.Structure):
+    _fields_ = [("count", C.c_int32), ("dtype", C.c_int32), ("params", C.c_void_p), ("grads", C.c_void_p), ("numel", C.c_void_p),
+                ("first_block", C.c_void_p), ("slots", C.c_void_p)]
 
 
 class TitaNetLibraryError(RuntimeError):
@@ -111,8 +126,9 @@ def load():
     lib.tn_grad_sumsq_partials.restype = i64
     lib.tn_grad_sumsq.argtypes = [i32, vp, vp, i32, vp, C.POINTER(i64), vp]
     lib.tn_grad_norm_finish.argtypes = [vp, i64, f64, f64, vp, vp, vp]
-    lib.tn_adamw_tick.argtypes = [i32, vp, vp, vp, vp, f64, vp, f64, f64, f64, vp]
-    lib.tn_adamw_apply.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64, vp, vp, f64, f64, f64, f64, vp]
+    lib.tn_adamw_tick.argtypes = [i32, vp, C.POINTER(TnAdamwState), C.POINTER(TnAdamwHyper), vp, i64, f64, f64, vp, vp, vp]
+    lib.tn_adamw_apply.argtypes = [C.POINTER(TnAdamwLists), C.POINTER(TnAdamwState), C.POINTER(TnAdamwHyper), f64, vp, vp]
+    lib.tn_adamw_step_small.argtypes = [C.POINTER(TnAdamwLists), C.POINTER(TnAdamwState), C.POINTER(TnAdamwHyper), i32, vp, f64, f64, vp, vp]
     lib.tn_moments_decode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
     lib.tn_moments_encode.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
     lib.tn_int8_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]

@@ -39,12 +39,13 @@ struct Lists {                         // the tensors of one type that a step to
   std::vector<const void*> g;
   std::vector<int64_t> numel, first;
   std::vector<int32_t> index, slot;
+  tn_adamw_lists c(int code) const { return {(int32_t)p.size(), code, p.data(), g.data(), numel.data(), first.data(), slot.data()}; }
 };
 
 struct GroupWork {
   std::array<Lists, 3> by_type;
   std::vector<int32_t> slots;
-  double lr, b1, b2, eps, wd;
+  tn_adamw_hyper h;
   at::Tensor lr_dev;
 };
 
@@ -146,33 +147,41 @@ class Stepper {
         }
     }
     void* stream = current_stream(dev);
-    const double* ctl = nullptr;
-    at::Tensor norm, ctl_mem, partials;
-    if (max_norm > 0.0) {
-      std::vector<std::pair<int, Lists*>> lists;
-      for (auto& w : work)
-        for (int code = 0; code < 3; ++code)
-          if (!w.by_type[code].p.empty()) lists.emplace_back(code, &w.by_type[code]);
-      partials = at::empty({Norm::partials(lists) + 2}, at::TensorOptions().dtype(at::kDouble).device(dev));
-      norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
-      double* mem = partials.mutable_data_ptr<double>();       // two for the factor, then the sums
-      const int64_t count = Norm::sums(lists, mem + 2, stream);
-      check(tn_grad_norm_finish(mem + 2, count, grad_mult, max_norm, norm.mutable_data_ptr<float>(), mem, stream), "tn_grad_norm_finish");
-      ctl = mem;
+    const tn_adamw_state state = {bits_, blocks_, exp_avg_.mutable_data_ptr(), exp_avg_sq_.mutable_data_ptr(),
+                                  scale1_.defined() ? scale1_.mutable_data_ptr<float>() : nullptr,
+                                  scale2_.defined() ? scale2_.mutable_data_ptr<float>() : nullptr, steps_.mutable_data_ptr<int32_t>(),
+                                  corr_.mutable_data_ptr<float>()};
+    std::vector<std::pair<int, Lists*>> lists;
+    for (auto& w : work)
+      for (int code = 0; code < 3; ++code)
+        if (!w.by_type[code].p.empty()) lists.emplace_back(code, &w.by_type[code]);
+    at::Tensor norm, partials;
+    if (max_norm > 0.0) norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    float* norm_ptr = norm.defined() ? norm.mutable_data_ptr<float>() : nullptr;
+    int small = TN_E_UNSUPPORTED;
+    if (lists.size() == 1) {
+      const tn_adamw_lists l = lists[0].second->c(lists[0].first);
+      small = tn_adamw_step_small(&l, &state, &work[0].h, (int32_t)work[0].slots.size(), work[0].slots.data(), grad_mult, max_norm, norm_ptr, stream);
+      if (small != TN_E_UNSUPPORTED) check(small, "tn_adamw_step_small");
     }
-    int32_t* steps = steps_.mutable_data_ptr<int32_t>();
-    float* corr = corr_.mutable_data_ptr<float>();
-    for (auto& w : work) {
-      check(tn_adamw_tick((int32_t)w.slots.size(), w.slots.data(), steps, corr, ctl, w.lr, w.lr_dev.defined() ? w.lr_dev.const_data_ptr<float>() : nullptr,
-                          w.b1, w.b2, w.wd, stream),
-            "tn_adamw_tick");
-      for (int code = 0; code < 3; ++code) {
-        Lists& l = w.by_type[code];
-        if (l.p.empty()) continue;
-        check(tn_adamw_apply((int32_t)l.p.size(), l.p.data(), l.g.data(), l.numel.data(), l.first.data(), l.slot.data(), code, bits_,
-                             exp_avg_.mutable_data_ptr(), exp_avg_sq_.mutable_data_ptr(), scale1_.defined() ? scale1_.mutable_data_ptr<float>() : nullptr,
-                             scale2_.defined() ? scale2_.mutable_data_ptr<float>() : nullptr, blocks_, corr, ctl, grad_mult, w.b1, w.b2, w.eps, stream),
-              "tn_adamw_apply");
+    if (small == TN_E_UNSUPPORTED) {
+      double* ctl = nullptr;
+      int64_t count = 0;
+      if (max_norm > 0.0) {
+        partials = at::empty({Norm::partials(lists) + 2}, at::TensorOptions().dtype(at::kDouble).device(dev));
+        ctl = partials.mutable_data_ptr<double>();             // two for the factor, then the sums
+        count = Norm::sums(lists, ctl + 2, stream);
+      }
+      bool first = max_norm > 0.0;
+      for (auto& w : work) {
+        check(tn_adamw_tick((int32_t)w.slots.size(), w.slots.data(), &state, &w.h, first ? ctl + 2 : nullptr, count, grad_mult, max_norm, norm_ptr, ctl, stream),
+              "tn_adamw_tick");
+        first = false;
+        for (int code = 0; code < 3; ++code) {
+          if (w.by_type[code].p.empty()) continue;
+          const tn_adamw_lists l = w.by_type[code].c(code);
+          check(tn_adamw_apply(&l, &state, &w.h, grad_mult, ctl, stream), "tn_adamw_apply");
+        }
       }
     }
     for (auto& p : stepped)
@@ -184,23 +193,25 @@ class Stepper {
  private:
   void hyper(const py::dict& group, const c10::Device& dev, bool capturing, GroupWork& w) {
     const py::object lr = group["lr"];
-    w.lr = 0.0;
+    w.h.lr = 0.0;
+    w.h.lr_dev = nullptr;
     if (THPVariable_Check(lr.ptr())) {
       w.lr_dev = THPVariable_Unpack(lr.ptr());
       TORCH_CHECK_VALUE(w.lr_dev.scalar_type() == at::kFloat && w.lr_dev.dim() == 0 && w.lr_dev.device() == dev,
                         "a tensor lr must be a 0-dim float32 tensor on the parameters' device");
+      w.h.lr_dev = w.lr_dev.const_data_ptr<float>();
     } else {
       TORCH_CHECK(!capturing, "AdamW: give lr as a 0-dim device tensor to capture a step (a number would be frozen into the graph)");
-      w.lr = lr.cast<double>();
-      TORCH_CHECK_VALUE(w.lr >= 0.0, "Invalid learning rate: ", w.lr);
+      w.h.lr = lr.cast<double>();
+      TORCH_CHECK_VALUE(w.h.lr >= 0.0, "Invalid learning rate: ", w.h.lr);
     }
     const py::sequence betas = group["betas"];
-    w.b1 = betas[0].cast<double>();
-    w.b2 = betas[1].cast<double>();
-    w.eps = group["eps"].cast<double>();
-    w.wd = group["weight_decay"].cast<double>();
-    TORCH_CHECK_VALUE(w.b1 >= 0.0 && w.b1 < 1.0 && w.b2 >= 0.0 && w.b2 < 1.0, "betas must be two numbers in [0, 1)");
-    TORCH_CHECK_VALUE(w.eps >= 0.0 && w.wd >= 0.0, "eps and weight_decay must not be negative");
+    w.h.beta1 = betas[0].cast<double>();
+    w.h.beta2 = betas[1].cast<double>();
+    w.h.eps = group["eps"].cast<double>();
+    w.h.weight_decay = group["weight_decay"].cast<double>();
+    TORCH_CHECK_VALUE(w.h.beta1 >= 0.0 && w.h.beta1 < 1.0 && w.h.beta2 >= 0.0 && w.h.beta2 < 1.0, "betas must be two numbers in [0, 1)");
+    TORCH_CHECK_VALUE(w.h.eps >= 0.0 && w.h.weight_decay >= 0.0, "eps and weight_decay must not be negative");
   }
 
   // Step counts belong to slots.  Where some of a slot's tensors have a gradient and others have not, those that have get a slot of

@@ -18,14 +18,14 @@ __device__ __forceinline__ int opt_find(const uint32_t* end, int count, uint32_t
   return __builtin_amdgcn_readfirstlane(t);
 }
 
-// four consecutive elements from i on, as floats; those from n on are 0 / not written.  The type's own alignment is enough.
+// four consecutive elements from i on, as floats; those from n on are 0 / not written (WHOLE: none are).  The type's own alignment is enough.
 template <typename T>
 struct OptVec {
   typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 };
-template <typename T>
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ void opt_load4(const T* p, int64_t i, int64_t n, float v[4]) {
-  if (i + 4 <= n) {
+  if (WHOLE || i + 4 <= n) {
     const typename OptVec<T>::type x = *reinterpret_cast<const typename OptVec<T>::type*>(p + i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (float)x[j];
@@ -34,9 +34,9 @@ __device__ __forceinline__ void opt_load4(const T* p, int64_t i, int64_t n, floa
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? (float)p[i + j] : 0.f;
   }
 }
-template <typename T>
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ void opt_store4(T* p, int64_t i, int64_t n, const float v[4]) {
-  if (i + 4 <= n) {
+  if (WHOLE || i + 4 <= n) {
     typename OptVec<T>::type x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
@@ -48,20 +48,31 @@ __device__ __forceinline__ void opt_store4(T* p, int64_t i, int64_t n, const flo
   }
 }
 
-// sum over a workgroup of 256, the same order every time; thread 0 has the result
+// sum over a workgroup of WAVES waves, the same order every time; thread 0 has the result
+template <int WAVES>
 __device__ __forceinline__ double opt_sum_workgroup(double s) {
-  __shared__ double part[4];
+  __shared__ double part[WAVES];
 #pragma unroll
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  return threadIdx.x == 0 ? (part[0] + part[1]) + (part[2] + part[3]) : 0.0;
+  double sum = 0.0;
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += part[w];
+  return sum;
 }
 
-__device__ __forceinline__ float opt_max_wave(float x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
-  return x;
+// largest of 64 lanes' numbers, the same in all lanes (a scalar)
+__device__ __forceinline__ uint32_t opt_max_wave(uint32_t x) {
+  auto up = [&](uint32_t y) { x = x > y ? x : y; };
+  up(__builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false));       // lane ^ 1
+  up(__builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, false));       // lane ^ 2
+  up(__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false));      // mirrored within 8
+  up(__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, false));      // mirrored within 16
+  up(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));      // lane 15 of rows 0, 2 to rows 1, 3
+  up(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));      // lane 31 to rows 2, 3: lane 63 has them all
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 // ---- 8-bit moments -------------------------------------------------------------------------------------------------------
@@ -82,16 +93,17 @@ __device__ __forceinline__ void opt_decode_first(uint32_t q, float scale, double
   const double s = (double)scale;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int c = (int8_t)(q >> (8 * j));
-    x[j] = ((double)(c < 0 ? -c * c : c * c) * (1.0 / 16129.0)) * s;
+    const float c = (float)(int8_t)(q >> (8 * j));
+    x[j] = ((double)(c * fabsf(c)) * (1.0 / 16129.0)) * s;             // 127^2
   }
 }
 __device__ __forceinline__ void opt_decode_second(uint32_t q, float scale, double x[4]) {
   const double s = (double)scale;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t c = (q >> (8 * j)) & 255u;
-    x[j] = ((double)(c * c * c * c) * (1.0 / 4228250625.0)) * s;      // 255^4, below 2^32
+    const float c = (float)((q >> (8 * j)) & 255u);
+    const double r = (double)(c * c);
+    x[j] = ((r * r) * (1.0 / 4228250625.0)) * s;                       // 255^4
   }
 }
 __device__ __forceinline__ double opt_ema(double b, double x, double w, double y) {
@@ -99,50 +111,134 @@ __device__ __forceinline__ double opt_ema(double b, double x, double w, double y
   const double p = b * x, q = w * y;
   return p + q;
 }
-// all 64 lanes of the wave call these, each with four of the block's 256 values; *scale is that of the block, infinity or NaN
-// if one of its values is
-__device__ __forceinline__ float opt_scale_wave(const double x[4]) {
-  float top = 0.f;
-  bool bad = false;
+// All 64 lanes of the wave call these, each with four of the block's 256 values and the same rounded to 32 bits.  *scale becomes
+// the block's; the bit pattern of a NaN or an infinity is above every finite one's, so the maximum finds them by itself.
+__device__ __forceinline__ float opt_scale_wave(const float f[4]) {
+  uint32_t top = 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = fabsf((float)x[j]);
-    bad |= !(a < __builtin_huge_valf());
-    top = fmaxf(top, a);
+    const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+    top = top > b ? top : b;
   }
   top = opt_max_wave(top);
-  return __ballot(bad) ? __builtin_nanf("") : top;
+  return top < 0x7f800000u ? __uint_as_float(top) : __builtin_nanf("");
 }
-__device__ __forceinline__ uint32_t opt_encode_first(const double x[4], float* scale) {
-  const float top = opt_scale_wave(x);
+// x / scale to float accuracy, for candidates; a scale whose reciprocal a float cannot hold goes through 64 bits
+__device__ __forceinline__ void opt_ratio(const double x[4], const float f[4], float scale, float r[4]) {
+  if (scale > 0x1p-100f) {             // (uniform over the wave)
+    const float inv = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = fabsf(f[j]) * inv;
+  } else {
+    const double inv = __builtin_amdgcn_rcp((double)scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = (float)(fabs(x[j]) * inv);
+  }
+}
+__device__ __forceinline__ uint32_t opt_encode_first(const double x[4], const float f[4], float* scale) {
+  const float top = opt_scale_wave(f);
   *scale = top;
   if (!(top > 0.f)) return 0u;
-  const double inv = __builtin_amdgcn_rcp((double)top), border = (double)top * (1.0 / 64516.0);       // (2 * 127)^2
+  float ratio[4];
+  opt_ratio(x, f, top, ratio);
+  const double border = (double)top * (1.0 / 64516.0);                 // (2 * 127)^2
   uint32_t q = 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double a = fabs(x[j]);
-    int c = (int)(127.f * __builtin_amdgcn_sqrtf((float)(a * inv)));
-    c = c < 126 ? c : 126;
-    c += a > (double)((2 * c + 1) * (2 * c + 1)) * border;
-    q |= (uint32_t)(uint8_t)(int8_t)(x[j] < 0.0 ? -c : c) << (8 * j);
+    float c = fminf(floorf(127.f * __builtin_amdgcn_sqrtf(ratio[j])), 126.f);
+    const float e = fmaf(2.f, c, 1.f);
+    c += fabs(x[j]) > (double)(e * e) * border ? 1.f : 0.f;
+    q = __builtin_amdgcn_cvt_pk_u8_f32(c, j, q);
   }
-  return q;
+  // negative values: two's complement of their byte, 0x80 - c with the top bit turned
+  const uint32_t neg = (0x80808080u - q) ^ 0x80808080u;
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x0c0c0b09u);      // 9, 11: a byte of sign bits
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x0b090c0cu);
+  const uint32_t mask = lo | hi;
+  return (neg & mask) | (q & ~mask);
 }
-__device__ __forceinline__ uint32_t opt_encode_second(const double x[4], float* scale) {
-  const float top = opt_scale_wave(x);
+__device__ __forceinline__ uint32_t opt_encode_second(const double x[4], const float f[4], float* scale) {
+  const float top = opt_scale_wave(f);
   *scale = top;
   if (!(top > 0.f)) return 0u;
-  const double inv = __builtin_amdgcn_rcp((double)top), border = (double)top * (1.0 / 67652010000.0);     // (2 * 255)^4
+  float ratio[4];
+  opt_ratio(x, f, top, ratio);
+  const double border = (double)top * (1.0 / 67652010000.0);           // (2 * 255)^4
   uint32_t q = 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    int c = (int)(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)(x[j] * inv))));
-    c = c < 254 ? c : 254;
-    const double r = (double)((2 * c + 1) * (2 * c + 1));
-    c += x[j] > r * r * border;
-    c = x[j] > 0.0 && c == 0 ? 1 : c;
-    q |= (uint32_t)c << (8 * j);
+    float c = fminf(floorf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(ratio[j]))), 254.f);
+    const float e = fmaf(2.f, c, 1.f);
+    const double r = (double)(e * e);
+    c += x[j] > (r * r) * border ? 1.f : 0.f;
+    c = fmaxf(c, x[j] > 0.0 ? 1.f : 0.f);
+    q = __builtin_amdgcn_cvt_pk_u8_f32(c, j, q);
   }
   return q;
+}
+
+// m / (sqrt(v) root + eps) with the hardware's root and reciprocal (one step of 32 bits each) where they hold; a root of a denormal
+// or a denominator of nothing goes the exact way
+__device__ __forceinline__ float opt_update(float m, float v, float root, float eps) {
+  const float d = fmaf(__builtin_amdgcn_sqrtf(v), root, eps);
+  if (d > 1e-18f && d < 1e18f) return m * __builtin_amdgcn_rcpf(d);
+  return m / (sqrtf(v) * root + eps);
+}
+
+struct OptStep {                       // what a step of one tensor needs besides its values
+  double b1, b2, w1, w2, factor;       // w = 1 - b
+  float rate, root, decay, eps;        // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+};
+
+// One block of 256 elements, four to a lane, from element i0 of a tensor of n on
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void opt_step8_block(const OptStep& h, T* p, const float g[4], int64_t i0, int64_t n, int64_t block, int8_t* exp_avg,
+                                                uint8_t* exp_avg_sq, float* scale1, float* scale2) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = i0 + 4 * lane;
+  float pv[4];
+  opt_load4<WHOLE>(p, i, n, pv);
+  uint32_t* q1 = reinterpret_cast<uint32_t*>(exp_avg + block * TN_OPT_BLOCK) + lane;
+  uint32_t* q2 = reinterpret_cast<uint32_t*>(exp_avg_sq + block * TN_OPT_BLOCK) + lane;
+  double m[4], v[4];
+  float mf[4], vf[4];
+  opt_decode_first(*q1, scale1[block], m);
+  opt_decode_second(*q2, scale2[block], v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const double gj = (double)g[j] * h.factor;
+    m[j] = opt_ema(h.b1, m[j], h.w1, gj);
+    v[j] = opt_ema(h.b2, v[j], h.w2, gj * gj);
+    mf[j] = (float)m[j];
+    vf[j] = (float)v[j];
+    pv[j] = pv[j] * h.decay - h.rate * opt_update(mf[j], vf[j], h.root, h.eps);
+  }
+  opt_store4<WHOLE>(p, i, n, pv);
+  float s1, s2;
+  const uint32_t n1 = opt_encode_first(m, mf, &s1), n2 = opt_encode_second(v, vf, &s2);
+  const bool bad = !(s1 < __builtin_huge_valf()) || !(s2 < __builtin_huge_valf());
+  *q1 = bad ? 0u : n1;
+  *q2 = bad ? 0u : n2;
+  if (lane == 0) {
+    scale1[block] = bad ? __builtin_nanf("") : s1;
+    scale2[block] = bad ? __builtin_nanf("") : s2;
+  }
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void opt_step32(const OptStep& h, T* p, const float g[4], int64_t i, int64_t n, float* m, float* v) {
+  const float b1 = (float)h.b1, b2 = (float)h.b2, w1 = (float)h.w1, w2 = (float)h.w2, factor = (float)h.factor;
+  float pv[4], mv[4], vv[4];
+  opt_load4<WHOLE>(p, i, n, pv);
+  opt_load4<WHOLE>(m, i, n, mv);              // (the padding of the last block is neither read nor written)
+  opt_load4<WHOLE>(v, i, n, vv);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float gj = g[j] * factor;
+    mv[j] = b1 * mv[j] + w1 * gj;
+    vv[j] = b2 * vv[j] + w2 * (gj * gj);
+    pv[j] = pv[j] * h.decay - h.rate * opt_update(mv[j], vv[j], h.root, h.eps);
+  }
+  opt_store4<WHOLE>(p, i, n, pv);
+  opt_store4<WHOLE>(m, i, n, mv);
+  opt_store4<WHOLE>(v, i, n, vv);
 }

@@ -14,7 +14,8 @@
 namespace {
 
 constexpr int OPT_CHUNK = 4096;        // elements of one workgroup of the step: 16 blocks of 256
-constexpr int SUM_CHUNK = 16384;       // elements behind one partial sum of the norm
+constexpr int SUM_CHUNK = 8192;        // elements behind one partial sum of the norm
+constexpr int SMALL_BLOCKS = 64;       // blocks of 256 that one workgroup steps by itself, norm and all
 constexpr int OPT_LIST = 96;           // tensors one launch can name in its arguments
 constexpr int64_t OPT_GRID = (1 << 24) - 1;      // workgroups of 256 in one launch: the grid is counted in 32 bits of threads
 
@@ -34,39 +35,39 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(SumList list, double* _
   const int64_t lo = (int64_t)(blockIdx.x - before) * SUM_CHUNK, n = list.numel[t];
   const T* g = reinterpret_cast<const T*>(list.g[t]);
   double s = 0.0;
-  for (int64_t i = lo + 4 * threadIdx.x; i < lo + SUM_CHUNK && i < n; i += 4 * 256) {
-    float v[4];
-    opt_load4(g, i, n, v);
+  float v[SUM_CHUNK / 1024][4];        // all loads of the chunk on their way together
+  if (lo + SUM_CHUNK <= n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
+    for (int k = 0; k < SUM_CHUNK / 1024; ++k) opt_load4<true>(g, lo + k * 1024 + 4 * threadIdx.x, n, v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < SUM_CHUNK / 1024; ++k) opt_load4(g, lo + k * 1024 + 4 * threadIdx.x, n, v[k]);
   }
-  s = opt_sum_workgroup(s);
+#pragma unroll
+  for (int k = 0; k < SUM_CHUNK / 1024; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = fma((double)v[k][j], (double)v[k][j], s);
+  s = opt_sum_workgroup<4>(s);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// norm = |mult| sqrt(sum), ctl = {factor of the gradients, 1 if the step runs}: a norm that is no number stops the step
-__global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* __restrict__ partials, int64_t count, double mult,
-                                                               double max_norm, float* __restrict__ norm_out, double* __restrict__ ctl) {
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < count; i += 256) s += partials[i];
-  s = opt_sum_workgroup(s);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(s) * fabs(mult);
-    if (norm_out) *norm_out = (float)norm;
-    if (ctl) {
-      const bool ok = norm < __builtin_huge_val();      // false for NaN too
-      const double c = max_norm / (norm + 1e-6);
-      ctl[0] = ok ? mult * (c < 1.0 ? c : 1.0) : 0.0;
-      ctl[1] = ok ? 1.0 : 0.0;
-    }
-  }
-}
-
-// -------------------------------------------------------------------------------------------------------------- the step
-struct OptSlots {
-  int32_t slot[256];
-  int32_t count;
+struct NormArgs {
+  const double* partials;
+  int64_t count;
+  double mult, max_norm;
+  float* norm;                         // may be null
+  double* ctl;                         // may be null
 };
+
+// norm = |mult| sqrt(sum), ctl = {factor of the gradients, 1 if the step runs}: a norm that is no number stops the step
+__device__ void opt_finish_norm(const NormArgs& a, double sum, double ctl[2]) {
+  const double norm = sqrt(sum) * fabs(a.mult);
+  if (a.norm) *a.norm = (float)norm;
+  const bool ok = norm < __builtin_huge_val();            // false for NaN too
+  const double c = a.max_norm / (norm + 1e-6);
+  ctl[0] = ok ? a.mult * (c < 1.0 ? c : 1.0) : 0.0;
+  ctl[1] = ok ? 1.0 : 0.0;
+}
 
 __device__ double opt_power(double b, int32_t t) {       // b^t by squaring: exact enough for 1 - b^t at every t
   double r = 1.0;
@@ -78,27 +79,70 @@ __device__ double opt_power(double b, int32_t t) {       // b^t by squaring: exa
   return r;
 }
 
+struct OptSlots {
+  int32_t slot[256];
+  int32_t count;
+};
+struct TickArgs {
+  int32_t* steps;
+  float* corr;
+  double lr;
+  const float* lr_dev;
+  double b1, b2, wd;
+};
+
 // steps[slot] += 1 and the four numbers of the step that depend on it: {step size, 1 / sqrt(1 - b2^t), 1 - lr wd, runs}
-__global__ __launch_bounds__(256) void adamw_tick_kernel(OptSlots list, int32_t* __restrict__ steps, float* __restrict__ corr,
-                                                         const double* __restrict__ ctl, double lr, const float* __restrict__ lr_dev,
-                                                         double b1, double b2, double wd) {
-  const int i = threadIdx.x;
-  if (i >= list.count) return;
-  const int s = list.slot[i];
-  float* c = corr + 4 * (int64_t)s;
-  if (ctl && ctl[1] == 0.0) {
-    c[3] = 0.f;
-    return;
+__device__ float4 opt_tick(const TickArgs& a, int slot, bool runs) {
+  float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (runs) {
+    const int32_t t = a.steps[slot] + 1;
+    a.steps[slot] = t;
+    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    c = make_float4((float)(lr / (1.0 - opt_power(a.b1, t))), (float)(1.0 / sqrt(1.0 - opt_power(a.b2, t))), (float)(1.0 - lr * a.wd), 1.f);
   }
-  const int32_t t = steps[s] + 1;
-  steps[s] = t;
-  if (lr_dev) lr = (double)*lr_dev;
-  c[0] = (float)(lr / (1.0 - opt_power(b1, t)));
-  c[1] = (float)(1.0 / sqrt(1.0 - opt_power(b2, t)));
-  c[2] = (float)(1.0 - lr * wd);
-  c[3] = 1.f;
+  reinterpret_cast<float4*>(a.corr)[slot] = c;
+  return c;
 }
 
+__device__ double opt_sum_partials(const NormArgs& a) {
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < a.count; i += 256) s += a.partials[i];
+  return opt_sum_workgroup<4>(s);
+}
+
+__global__ __launch_bounds__(256) void grad_norm_finish_kernel(NormArgs a) {
+  const double s = opt_sum_partials(a);
+  double ctl[2];
+  if (threadIdx.x == 0) {
+    opt_finish_norm(a, s, ctl);
+    if (a.ctl) {
+      a.ctl[0] = ctl[0];
+      a.ctl[1] = ctl[1];
+    }
+  }
+}
+
+// The norm's end (first = true: from its partial sums; otherwise ctl has it) and the counts, in one launch
+__global__ __launch_bounds__(256) void adamw_tick_kernel(OptSlots list, TickArgs t, NormArgs a, bool first) {
+  __shared__ double runs;
+  if (first) {
+    const double s = opt_sum_partials(a);
+    double ctl[2];
+    if (threadIdx.x == 0) {
+      opt_finish_norm(a, s, ctl);
+      a.ctl[0] = ctl[0];
+      a.ctl[1] = ctl[1];
+      runs = ctl[1];
+    }
+    __syncthreads();
+  } else if (threadIdx.x == 0) {
+    runs = a.ctl ? a.ctl[1] : 1.0;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < list.count) opt_tick(t, list.slot[threadIdx.x], runs != 0.0);
+}
+
+// -------------------------------------------------------------------------------------------------------------- the step
 struct OptList {
   void* p[OPT_LIST];
   const void* g[OPT_LIST];
@@ -114,36 +158,37 @@ struct OptHyper {
   double mult;                         // factor of the gradients where ctl is null
 };
 
+__device__ __forceinline__ OptStep opt_step_of(const OptHyper& h, const float4& c, double factor) {
+  return {h.b1, h.b2, h.w1, h.w2, factor, c.x, c.y, c.z, h.eps};
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, float* __restrict__ exp_avg, float* __restrict__ exp_avg_sq,
                                                       const float* __restrict__ corr, const double* __restrict__ ctl) {
   const int t = opt_find(list.end, OPT_LIST, blockIdx.x);
-  const float4 c = *reinterpret_cast<const float4*>(corr + 4 * (int64_t)list.slot[t]);
+  const float4 c = reinterpret_cast<const float4*>(corr)[list.slot[t]];
   if (c.w == 0.f) return;
-  const float factor = (float)(ctl ? ctl[0] : h.mult);
-  const float b1 = (float)h.b1, b2 = (float)h.b2, w1 = (float)h.w1, w2 = (float)h.w2;
+  const OptStep step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
   const uint32_t before = t ? list.end[t - 1] : 0u;
   const int64_t lo = (int64_t)(blockIdx.x - before) * OPT_CHUNK, n = list.numel[t];
   T* p = reinterpret_cast<T*>(list.p[t]);
   const T* g = reinterpret_cast<const T*>(list.g[t]);
   float* m = exp_avg + (int64_t)list.first_block[t] * TN_OPT_BLOCK;
   float* v = exp_avg_sq + (int64_t)list.first_block[t] * TN_OPT_BLOCK;
-  for (int64_t i = lo + 4 * threadIdx.x; i < lo + OPT_CHUNK && i < n; i += 4 * 256) {
-    float pv[4], gv[4], mv[4], vv[4];
-    opt_load4(p, i, n, pv);
-    opt_load4(g, i, n, gv);
-    opt_load4(m, i, n, mv);            // (the padding of the last block is read and written as zeros)
-    opt_load4(v, i, n, vv);
+  if (lo + OPT_CHUNK <= n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float gj = gv[j] * factor;
-      mv[j] = b1 * mv[j] + w1 * gj;
-      vv[j] = b2 * vv[j] + w2 * (gj * gj);
-      pv[j] = pv[j] * c.z - c.x * (mv[j] / (sqrtf(vv[j]) * c.y + h.eps));
+    for (int k = 0; k < OPT_CHUNK / 1024; ++k) {
+      const int64_t i = lo + k * 1024 + 4 * threadIdx.x;
+      float gv[4];
+      opt_load4<true>(g, i, n, gv);
+      opt_step32<true>(step, p, gv, i, n, m, v);
     }
-    opt_store4(p, i, n, pv);
-    opt_store4(m, i, n, mv);
-    opt_store4(v, i, n, vv);
+  } else {
+    for (int64_t i = lo + 4 * threadIdx.x; i < n; i += 1024) {
+      float gv[4];
+      opt_load4(g, i, n, gv);
+      opt_step32<false>(step, p, gv, i, n, m, v);
+    }
   }
 }
 
@@ -154,43 +199,74 @@ __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, i
                                                      float* __restrict__ scale1, float* __restrict__ scale2,
                                                      const float* __restrict__ corr, const double* __restrict__ ctl) {
   const int t = opt_find(list.end, OPT_LIST, blockIdx.x);
-  const float4 c = *reinterpret_cast<const float4*>(corr + 4 * (int64_t)list.slot[t]);
+  const float4 c = reinterpret_cast<const float4*>(corr)[list.slot[t]];
   if (c.w == 0.f) return;
-  const double factor = ctl ? ctl[0] : h.mult;
+  const OptStep step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
   const uint32_t before = t ? list.end[t - 1] : 0u;
   const int64_t lo = (int64_t)(blockIdx.x - before) * OPT_CHUNK, n = list.numel[t];
   T* p = reinterpret_cast<T*>(list.p[t]);
   const T* g = reinterpret_cast<const T*>(list.g[t]);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int k = wave; k < OPT_CHUNK / TN_OPT_BLOCK; k += 4) {
-    const int64_t i0 = lo + (int64_t)k * TN_OPT_BLOCK, i = i0 + 4 * lane;
+  for (int k = threadIdx.x >> 6; k < OPT_CHUNK / TN_OPT_BLOCK; k += 4) {
+    const int64_t i0 = lo + (int64_t)k * TN_OPT_BLOCK;
     if (i0 >= n) break;
-    const int64_t block = (int64_t)list.first_block[t] + i0 / TN_OPT_BLOCK;
-    float pv[4], gv[4];
-    opt_load4(p, i, n, pv);
-    opt_load4(g, i, n, gv);
-    uint32_t* q1 = reinterpret_cast<uint32_t*>(exp_avg + block * TN_OPT_BLOCK) + lane;
-    uint32_t* q2 = reinterpret_cast<uint32_t*>(exp_avg_sq + block * TN_OPT_BLOCK) + lane;
-    double m[4], v[4];
-    opt_decode_first(*q1, scale1[block], m);
-    opt_decode_second(*q2, scale2[block], v);
+    const int64_t i = i0 + 4 * (threadIdx.x & 63), block = (int64_t)list.first_block[t] + i0 / TN_OPT_BLOCK;
+    float gv[4];
+    if (i0 + TN_OPT_BLOCK <= n) {
+      opt_load4<true>(g, i, n, gv);
+      opt_step8_block<true>(step, p, gv, i0, n, block, exp_avg, exp_avg_sq, scale1, scale2);
+    } else {
+      opt_load4(g, i, n, gv);
+      opt_step8_block<false>(step, p, gv, i0, n, block, exp_avg, exp_avg_sq, scale1, scale2);
+    }
+  }
+}
+
+// A few small tensors: one workgroup of 16 waves takes the norm, the counts and the step, a block of 256 elements to a wave and turn
+// with its gradient kept in registers in between.  Where the launches of the general way (norm, counts, step) take 20 us, this
+// one takes 7 up to SMALL_BLOCKS blocks.
+template <typename T, int BITS>
+__global__ __launch_bounds__(1024) void adamw_small_kernel(OptList list, OptHyper h, OptSlots slots, TickArgs tick, NormArgs a, bool clip, void* exp_avg,
+                                                           void* exp_avg_sq, float* scale1, float* scale2) {
+  constexpr int TURNS = SMALL_BLOCKS / 16;
+  __shared__ double ctl[2];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float g[TURNS][4];
+  double s = 0.0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double gj = (double)gv[j] * factor;
-      m[j] = opt_ema(h.b1, m[j], h.w1, gj);
-      v[j] = opt_ema(h.b2, v[j], h.w2, gj * gj);
-      pv[j] = pv[j] * c.z - c.x * ((float)m[j] / (sqrtf((float)v[j]) * c.y + h.eps));
-    }
-    opt_store4(p, i, n, pv);
-    float s1, s2;
-    const uint32_t n1 = opt_encode_first(m, &s1), n2 = opt_encode_second(v, &s2);
-    const bool bad = !(s1 < __builtin_huge_valf()) || !(s2 < __builtin_huge_valf());
-    *q1 = n1;
-    *q2 = n2;
-    if (lane == 0) {
-      scale1[block] = bad ? __builtin_nanf("") : s1;
-      scale2[block] = bad ? __builtin_nanf("") : s2;
-    }
+  for (int k = 0; k < TURNS; ++k) {                 // (end counts blocks here)
+    const uint32_t b = k * 16 + wave;
+    const int t = opt_find(list.end, OPT_LIST, b);
+    if (t >= OPT_LIST || list.end[t] == 0xffffffffu) continue;
+    const int64_t i0 = (int64_t)(b - (t ? list.end[t - 1] : 0u)) * TN_OPT_BLOCK;
+    opt_load4(reinterpret_cast<const T*>(list.g[t]), i0 + 4 * lane, list.numel[t], g[k]);
+    if (clip)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fma((double)g[k][j], (double)g[k][j], s);
+  }
+  if (clip) {
+    s = opt_sum_workgroup<16>(s);
+    if (threadIdx.x == 0) opt_finish_norm(a, s, ctl);
+  } else if (threadIdx.x == 0) {
+    ctl[0] = h.mult;
+    ctl[1] = 1.0;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < slots.count) opt_tick(tick, slots.slot[threadIdx.x], ctl[1] != 0.0);
+  __syncthreads();                                  // (corr is this workgroup's own writing: visible behind the barrier)
+  if (ctl[1] == 0.0) return;
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    const uint32_t b = k * 16 + wave;
+    const int t = opt_find(list.end, OPT_LIST, b);
+    if (t >= OPT_LIST || list.end[t] == 0xffffffffu) continue;
+    const float4 c = reinterpret_cast<const float4*>(tick.corr)[list.slot[t]];
+    const OptStep step = opt_step_of(h, c, ctl[0]);
+    const int64_t i0 = (int64_t)(b - (t ? list.end[t - 1] : 0u)) * TN_OPT_BLOCK, first = list.first_block[t];
+    T* p = reinterpret_cast<T*>(list.p[t]);
+    if constexpr (BITS == 32)
+      opt_step32<false>(step, p, g[k], i0 + 4 * lane, list.numel[t], (float*)exp_avg + first * TN_OPT_BLOCK, (float*)exp_avg_sq + first * TN_OPT_BLOCK);
+    else
+      opt_step8_block<false>(step, p, g[k], i0, list.numel[t], first + i0 / TN_OPT_BLOCK, (int8_t*)exp_avg, (uint8_t*)exp_avg_sq, scale1, scale2);
   }
 }
 
@@ -213,12 +289,13 @@ __global__ __launch_bounds__(256) void moments_encode_kernel(const float* __rest
   const int lane = threadIdx.x & 63;
   for (int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (int64_t)gridDim.x * 4) {
   const float4 a = reinterpret_cast<const float4*>(m + b * TN_OPT_BLOCK)[lane], c = reinterpret_cast<const float4*>(v + b * TN_OPT_BLOCK)[lane];
+  const float xf[4] = {a.x, a.y, a.z, a.w}, yf[4] = {c.x, c.y, c.z, c.w};
   const double x[4] = {a.x, a.y, a.z, a.w}, y[4] = {c.x, c.y, c.z, c.w};
   float s1, s2;
-  const uint32_t n1 = opt_encode_first(x, &s1), n2 = opt_encode_second(y, &s2);
+  const uint32_t n1 = opt_encode_first(x, xf, &s1), n2 = opt_encode_second(y, yf, &s2);
   const bool bad = !(s1 < __builtin_huge_valf()) || !(s2 < __builtin_huge_valf());
-  reinterpret_cast<uint32_t*>(q1 + b * TN_OPT_BLOCK)[lane] = n1;
-  reinterpret_cast<uint32_t*>(q2 + b * TN_OPT_BLOCK)[lane] = n2;
+  reinterpret_cast<uint32_t*>(q1 + b * TN_OPT_BLOCK)[lane] = bad ? 0u : n1;
+  reinterpret_cast<uint32_t*>(q2 + b * TN_OPT_BLOCK)[lane] = bad ? 0u : n2;
   if (lane == 0) {
     scale1[b] = bad ? __builtin_nanf("") : s1;
     scale2[b] = bad ? __builtin_nanf("") : s2;
@@ -296,82 +373,148 @@ extern "C" int tn_grad_sumsq(int32_t count, const void* const* grads, const int6
 extern "C" int tn_grad_norm_finish(const double* partials, int64_t count, double grad_mult, double max_norm, float* norm, double* ctl,
                                    void* stream) {
   if (count < 0 || (count > 0 && !partials) || (!norm && !ctl) || (ctl && !(max_norm > 0.0))) return TN_E_BADARG;
-  hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, partials, count, grad_mult, max_norm, norm, ctl);
+  const NormArgs a = {partials, count, grad_mult, max_norm, norm, ctl};
+  hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 
-extern "C" int tn_adamw_tick(int32_t count, const int32_t* slots, int32_t* steps, float* corr, const double* ctl, double lr,
-                             const float* lr_dev, double beta1, double beta2, double weight_decay, void* stream) {
-  if (count < 0 || (count > 0 && (!slots || !steps || !corr))) return TN_E_BADARG;
-  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || (!lr_dev && !(lr >= 0.0)) || !(weight_decay >= 0.0)) return TN_E_BADARG;
+namespace {
+
+bool hyper_ok(const tn_adamw_hyper* h) {
+  return h && h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0 && h->weight_decay >= 0.0 &&
+         (h->lr_dev || h->lr >= 0.0);
+}
+OptHyper hyper_of(const tn_adamw_hyper* h, double mult) { return {h->beta1, h->beta2, 1.0 - h->beta1, 1.0 - h->beta2, (float)h->eps, mult}; }
+TickArgs tick_of(const tn_adamw_hyper* h, int32_t* steps, float* corr) { return {steps, corr, h->lr, h->lr_dev, h->beta1, h->beta2, h->weight_decay}; }
+
+int lists_ok(const tn_adamw_lists* l, const tn_adamw_state* s) {
+  if (!l || !s || l->count < 0) return TN_E_BADARG;
+  if (l->dtype < TN_DTYPE_F32 || l->dtype > TN_DTYPE_F16 || (s->bits != 8 && s->bits != 32)) return TN_E_UNSUPPORTED;
+  if (s->blocks < 0 || s->blocks > 0xffffffffll) return TN_E_UNSUPPORTED;
+  if (l->count == 0) return 0;
+  if (!l->params || !l->grads || !l->numel || !l->first_block || !l->slots || !s->exp_avg || !s->exp_avg_sq || !s->corr) return TN_E_BADARG;
+  if (s->bits == 8 && (!s->scale1 || !s->scale2)) return TN_E_BADARG;
+  for (int i = 0; i < l->count; ++i)
+    if (l->numel[i] < 0 || (l->numel[i] > 0 && (!l->params[i] || !l->grads[i])) || l->slots[i] < 0 || l->first_block[i] < 0 ||
+        l->numel[i] > (s->blocks - l->first_block[i]) * TN_OPT_BLOCK)
+      return TN_E_BADARG;
+  return 0;
+}
+
+// Runs of the list, tensors that follow one another in parameters, gradients and moments joined: f(first of the run, elements).
+template <typename F>
+int each_run(const tn_adamw_lists* l, F f) {
+  const size_t size = opt_size(l->dtype);
+  for (int i = 0; i < l->count;) {
+    const int a = i++;
+    int64_t n = l->numel[a];
+    if (n == 0) continue;
+    while (i < l->count && l->numel[i] > 0 && l->slots[i] == l->slots[a] &&
+           l->first_block[i] * TN_OPT_BLOCK == l->first_block[a] * TN_OPT_BLOCK + n && opt_follows(l->params[a], n, size, l->params[i]) &&
+           opt_follows(l->grads[a], n, size, l->grads[i]))
+      n += l->numel[i++];
+    if (const int rc = f(a, n)) return rc;
+  }
+  return 0;
+}
+
+void put_run(OptList& list, int at, const tn_adamw_lists* l, int a, int64_t n, uint32_t end) {
+  list.p[at] = l->params[a];
+  list.g[at] = l->grads[a];
+  list.numel[at] = n;
+  list.first_block[at] = (uint32_t)l->first_block[a];
+  list.slot[at] = (uint32_t)l->slots[a];
+  list.end[at] = end;
+}
+
+}  // namespace
+
+extern "C" int tn_adamw_tick(int32_t count, const int32_t* slots, const tn_adamw_state* s, const tn_adamw_hyper* h, const double* partials,
+                             int64_t n_partials, double grad_mult, double max_norm, float* norm, double* ctl, void* stream) {
+  if (count < 0 || !s || !hyper_ok(h) || (count > 0 && (!slots || !s->steps || !s->corr))) return TN_E_BADARG;
+  if (partials && (n_partials < 0 || !ctl || !(max_norm > 0.0))) return TN_E_BADARG;
+  for (int i = 0; i < count; ++i)
+    if (slots[i] < 0) return TN_E_BADARG;
+  const NormArgs a = {partials, n_partials, grad_mult, max_norm, norm, ctl};
   for (int lo = 0; lo < count; lo += 256) {
-    OptSlots s;
-    s.count = std::min(256, count - lo);
-    for (int i = 0; i < s.count; ++i) {
-      if (slots[lo + i] < 0) return TN_E_BADARG;
-      s.slot[i] = slots[lo + i];
-    }
-    hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, s, steps, corr, ctl, lr, lr_dev, beta1, beta2, weight_decay);
+    OptSlots list;
+    list.count = std::min(256, count - lo);
+    for (int i = 0; i < list.count; ++i) list.slot[i] = slots[lo + i];
+    hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, list, tick_of(h, s->steps, s->corr), a, partials && lo == 0);
     if (const int rc = (int)hipGetLastError()) return rc;
   }
   return 0;
 }
 
-extern "C" int tn_adamw_apply(int32_t count, void* const* params, const void* const* grads, const int64_t* numel, const int64_t* first_block,
-                              const int32_t* slots, int32_t dtype, int32_t state_bits, void* exp_avg, void* exp_avg_sq, float* scale1,
-                              float* scale2, int64_t blocks, const float* corr, const double* ctl, double grad_mult, double beta1,
-                              double beta2, double eps, void* stream) {
-  if (count < 0 || (count > 0 && (!params || !grads || !numel || !first_block || !slots || !exp_avg || !exp_avg_sq || !corr))) return TN_E_BADARG;
-  if (dtype < TN_DTYPE_F32 || dtype > TN_DTYPE_F16 || (state_bits != 8 && state_bits != 32)) return TN_E_UNSUPPORTED;
-  if (count > 0 && state_bits == 8 && (!scale1 || !scale2)) return TN_E_BADARG;
-  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0)) return TN_E_BADARG;
-  if (blocks < 0 || blocks > 0xffffffffll) return TN_E_UNSUPPORTED;
-  for (int i = 0; i < count; ++i)
-    if (numel[i] < 0 || (numel[i] > 0 && (!params[i] || !grads[i])) || slots[i] < 0 || first_block[i] < 0 ||
-        first_block[i] + (numel[i] + TN_OPT_BLOCK - 1) / TN_OPT_BLOCK > blocks)
-      return TN_E_BADARG;
-  const OptHyper h = {beta1, beta2, 1.0 - beta1, 1.0 - beta2, (float)eps, grad_mult};
-  const size_t size = opt_size(dtype);
+extern "C" int tn_adamw_apply(const tn_adamw_lists* l, const tn_adamw_state* s, const tn_adamw_hyper* h, double grad_mult, const double* ctl,
+                              void* stream) {
+  if (!hyper_ok(h)) return TN_E_BADARG;
+  if (const int rc = lists_ok(l, s)) return rc;
   OptList list;
   int used = 0;
   uint32_t chunks = 0;
   auto flush = [&]() -> int {
     if (!used) return 0;
     for (int i = used; i < OPT_LIST; ++i) list.end[i] = 0xffffffffu;
-    const int rc = opt_by_type(dtype, [&](auto* kind) -> int {
+    const int rc = opt_by_type(l->dtype, [&](auto* kind) -> int {
       using T = std::remove_pointer_t<decltype(kind)>;
-      if (state_bits == 32)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw32_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, h, (float*)exp_avg,
-                           (float*)exp_avg_sq, corr, ctl);
+      if (s->bits == 32)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw32_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult),
+                           (float*)s->exp_avg, (float*)s->exp_avg_sq, s->corr, ctl);
       else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw8_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, h, (int8_t*)exp_avg,
-                           (uint8_t*)exp_avg_sq, scale1, scale2, corr, ctl);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw8_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult),
+                           (int8_t*)s->exp_avg, (uint8_t*)s->exp_avg_sq, s->scale1, s->scale2, s->corr, ctl);
       return (int)hipGetLastError();
     });
     used = 0;
     chunks = 0;
     return rc;
   };
-  for (int i = 0; i < count;) {
-    const int a = i++;
-    int64_t n = numel[a];
-    if (n == 0) continue;
-    while (i < count && numel[i] > 0 && slots[i] == slots[a] && first_block[i] * TN_OPT_BLOCK == first_block[a] * TN_OPT_BLOCK + n &&
-           opt_follows(params[a], n, size, params[i]) && opt_follows(grads[a], n, size, grads[i]))
-      n += numel[i++];
+  const int rc = each_run(l, [&](int a, int64_t n) -> int {
     const int64_t c = (n + OPT_CHUNK - 1) / OPT_CHUNK;
     if (c > OPT_GRID) return TN_E_UNSUPPORTED;
     if (used == OPT_LIST || (int64_t)chunks + c > OPT_GRID)
-      if (const int rc = flush()) return rc;
-    list.p[used] = params[a];
-    list.g[used] = grads[a];
-    list.numel[used] = n;
-    list.first_block[used] = (uint32_t)first_block[a];
-    list.slot[used] = (uint32_t)slots[a];
+      if (const int e = flush()) return e;
     chunks += (uint32_t)c;
-    list.end[used++] = chunks;
+    put_run(list, used++, l, a, n, chunks);
+    return 0;
+  });
+  return rc ? rc : flush();
+}
+
+extern "C" int tn_adamw_step_small(const tn_adamw_lists* l, const tn_adamw_state* s, const tn_adamw_hyper* h, int32_t n_slots, const int32_t* slots,
+                                   double grad_mult, double max_norm, float* norm, void* stream) {
+  if (!hyper_ok(h) || n_slots < 0 || (n_slots > 0 && !slots) || max_norm < 0.0) return TN_E_BADARG;
+  if (const int rc = lists_ok(l, s)) return rc;
+  if (!s->steps || n_slots > 256) return s->steps ? TN_E_UNSUPPORTED : TN_E_BADARG;
+  OptSlots sl;
+  sl.count = n_slots;
+  for (int i = 0; i < n_slots; ++i) {
+    if (slots[i] < 0) return TN_E_BADARG;
+    sl.slot[i] = slots[i];
   }
-  return flush();
+  OptList list;
+  int used = 0;
+  uint32_t blocks = 0;
+  const int rc = each_run(l, [&](int a, int64_t n) -> int {
+    const int64_t c = (n + TN_OPT_BLOCK - 1) / TN_OPT_BLOCK;
+    if (used == OPT_LIST || c > SMALL_BLOCKS || blocks + c > SMALL_BLOCKS) return TN_E_UNSUPPORTED;
+    blocks += (uint32_t)c;
+    put_run(list, used++, l, a, n, blocks);
+    return 0;
+  });
+  if (rc) return rc;
+  for (int i = used; i < OPT_LIST; ++i) list.end[i] = 0xffffffffu;
+  const NormArgs a = {nullptr, 0, grad_mult, max_norm, norm, nullptr};
+  return opt_by_type(l->dtype, [&](auto* kind) -> int {
+    using T = std::remove_pointer_t<decltype(kind)>;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult), sl, tick_of(h, s->steps, s->corr), a,
+                         max_norm > 0.0, s->exp_avg, s->exp_avg_sq, s->scale1, s->scale2);
+      return (int)hipGetLastError();
+    };
+    return s->bits == 32 ? go(adamw_small_kernel<T, 32>) : go(adamw_small_kernel<T, 8>);
+  });
 }
 
 extern "C" int tn_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale1, const float* scale2, float* out1,
