@@ -39,6 +39,14 @@ struct Lists {                         // the tensors of one type that a step to
   std::vector<const void*> g;
   std::vector<int64_t> numel, first;
   std::vector<int32_t> index, slot;
+  void reserve(size_t n) {
+    p.reserve(n);
+    g.reserve(n);
+    numel.reserve(n);
+    first.reserve(n);
+    index.reserve(n);
+    slot.reserve(n);
+  }
   tn_adamw_lists c(int code) const { return {(int32_t)p.size(), code, p.data(), g.data(), numel.data(), first.data(), slot.data()}; }
 };
 
@@ -88,13 +96,27 @@ class Stepper {
     slots_ = std::move(s);
   }
 
+  // the moments as float32 values; 32 bits: the buffers themselves
+  std::pair<at::Tensor, at::Tensor> moments() const {
+    if (bits_ == 32) return {exp_avg_, exp_avg_sq_};
+    const at::NoGradGuard no_grad;
+    const c10::OptionalDeviceGuard guard(exp_avg_.device());
+    at::Tensor m = at::empty(exp_avg_.sizes(), scale1_.options()), v = at::empty(exp_avg_.sizes(), scale1_.options());
+    check(tn_moments_decode(exp_avg_.const_data_ptr(), exp_avg_sq_.const_data_ptr(), scale1_.const_data_ptr<float>(), scale2_.const_data_ptr<float>(),
+                            m.mutable_data_ptr<float>(), v.mutable_data_ptr<float>(), blocks_, current_stream(exp_avg_.device())),
+          "tn_moments_decode");
+    return {m, v};
+  }
+
   // one step of all groups; the norm before clipping (0-dim float32) where max_norm > 0
   std::optional<at::Tensor> step(const py::list& groups, double max_norm, double grad_mult) {
     const at::NoGradGuard no_grad;
     const c10::Device dev = exp_avg_.device();
     const c10::OptionalDeviceGuard guard(dev);
     const bool capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
-    std::vector<at::Tensor> keep, stepped;       // gradients laid out anew; parameters
+    std::vector<at::Tensor> keep;                // gradients laid out anew
+    std::vector<c10::TensorImpl*> stepped;       // parameters (the group's list holds them)
+    stepped.reserve(numel_.size());
     std::vector<GroupWork> work;
     std::vector<char> active(numel_.size(), 0);
     work.reserve(groups.size());
@@ -104,10 +126,12 @@ class Stepper {
       const py::list params = group["params"];
       GroupWork w;
       bool any = false;
-      for (const auto& obj : params) {
+      const Py_ssize_t count = PyList_GET_SIZE(params.ptr());
+      for (Py_ssize_t k = 0; k < count; ++k) {
+        PyObject* obj = PyList_GET_ITEM(params.ptr(), k);
         const int32_t i = at++;
-        TORCH_CHECK(THPVariable_Check(obj.ptr()) && (size_t)i < numel_.size(), "AdamW: the parameter list changed; use add_param_group");
-        const at::Tensor& p = THPVariable_Unpack(obj.ptr());
+        TORCH_CHECK(THPVariable_Check(obj) && (size_t)i < numel_.size(), "AdamW: the parameter list changed; use add_param_group");
+        const at::Tensor& p = THPVariable_Unpack(obj);
         const at::Tensor& given = p.grad();
         if (!given.defined()) continue;
         TORCH_CHECK(given.layout() == at::kStrided, "AdamW does not take sparse gradients");
@@ -122,6 +146,7 @@ class Stepper {
           g = keep.back().const_data_ptr();
         }
         Lists& l = w.by_type[code];
+        if (l.p.empty()) l.reserve((size_t)count);
         l.p.push_back(p.mutable_data_ptr());
         l.g.push_back(g);
         l.numel.push_back(numel_[i]);
@@ -129,7 +154,7 @@ class Stepper {
         l.index.push_back(i);
         active[i] = 1;
         any = true;
-        stepped.push_back(p);
+        stepped.push_back(p.unsafeGetTensorImpl());
       }
       if (!any) continue;
       hyper(group, dev, capturing, w);
@@ -184,8 +209,8 @@ class Stepper {
         }
       }
     }
-    for (auto& p : stepped)
-      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();      // autograd has to see that the values changed
+    for (c10::TensorImpl* p : stepped)
+      if (!p->is_inference()) p->bump_version();      // autograd has to see that the values changed
     if (max_norm > 0.0) return norm;
     return std::nullopt;
   }
@@ -362,6 +387,7 @@ PYBIND11_MODULE(_host, m) {
       .def(py::init<int>())
       .def("layout", &Stepper::layout)
       .def("step", &Stepper::step)
+      .def("moments", &Stepper::moments)
       .def_property("slots", &Stepper::slots, &Stepper::set_slots);
   m.def("grad_norm", &grad_norm);
   m.def("quantize_rows", &quantize_rows);

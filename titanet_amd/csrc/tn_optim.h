@@ -23,10 +23,12 @@ template <typename T>
 struct OptVec {
   typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 };
-template <bool WHOLE = false, typename T>
+// ONCE: nothing reads these lines again before the next step, they need not stay in a cache.
+template <bool WHOLE = false, bool ONCE = false, typename T>
 __device__ __forceinline__ void opt_load4(const T* p, int64_t i, int64_t n, float v[4]) {
   if (WHOLE || i + 4 <= n) {
-    const typename OptVec<T>::type x = *reinterpret_cast<const typename OptVec<T>::type*>(p + i);
+    const typename OptVec<T>::type* at = reinterpret_cast<const typename OptVec<T>::type*>(p + i);
+    const typename OptVec<T>::type x = ONCE ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (float)x[j];
   } else {
@@ -34,13 +36,15 @@ __device__ __forceinline__ void opt_load4(const T* p, int64_t i, int64_t n, floa
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? (float)p[i + j] : 0.f;
   }
 }
-template <bool WHOLE = false, typename T>
+template <bool WHOLE = false, bool ONCE = false, typename T>
 __device__ __forceinline__ void opt_store4(T* p, int64_t i, int64_t n, const float v[4]) {
   if (WHOLE || i + 4 <= n) {
     typename OptVec<T>::type x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
-    *reinterpret_cast<typename OptVec<T>::type*>(p + i) = x;
+    typename OptVec<T>::type* at = reinterpret_cast<typename OptVec<T>::type*>(p + i);
+    if constexpr (ONCE) __builtin_nontemporal_store(x, at);
+    else *at = x;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -202,8 +206,8 @@ __device__ __forceinline__ void opt_step8_block(const OptStep& h, T* p, const fl
   uint32_t* q2 = reinterpret_cast<uint32_t*>(exp_avg_sq + block * TN_OPT_BLOCK) + lane;
   double m[4], v[4];
   float mf[4], vf[4];
-  opt_decode_first(*q1, scale1[block], m);
-  opt_decode_second(*q2, scale2[block], v);
+  opt_decode_first(__builtin_nontemporal_load(q1), scale1[block], m);
+  opt_decode_second(__builtin_nontemporal_load(q2), scale2[block], v);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double gj = (double)g[j] * h.factor;
@@ -217,8 +221,8 @@ __device__ __forceinline__ void opt_step8_block(const OptStep& h, T* p, const fl
   float s1, s2;
   const uint32_t n1 = opt_encode_first(m, mf, &s1), n2 = opt_encode_second(v, vf, &s2);
   const bool bad = !(s1 < __builtin_huge_valf()) || !(s2 < __builtin_huge_valf());
-  *q1 = bad ? 0u : n1;
-  *q2 = bad ? 0u : n2;
+  __builtin_nontemporal_store(bad ? 0u : n1, q1);
+  __builtin_nontemporal_store(bad ? 0u : n2, q2);
   if (lane == 0) {
     scale1[block] = bad ? __builtin_nanf("") : s1;
     scale2[block] = bad ? __builtin_nanf("") : s2;
@@ -229,8 +233,8 @@ __device__ __forceinline__ void opt_step32(const OptStep& h, T* p, const float g
   const float b1 = (float)h.b1, b2 = (float)h.b2, w1 = (float)h.w1, w2 = (float)h.w2, factor = (float)h.factor;
   float pv[4], mv[4], vv[4];
   opt_load4<WHOLE>(p, i, n, pv);
-  opt_load4<WHOLE>(m, i, n, mv);              // (the padding of the last block is neither read nor written)
-  opt_load4<WHOLE>(v, i, n, vv);
+  opt_load4<WHOLE, true>(m, i, n, mv);              // (the padding of the last block is neither read nor written)
+  opt_load4<WHOLE, true>(v, i, n, vv);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float gj = g[j] * factor;
@@ -239,6 +243,6 @@ __device__ __forceinline__ void opt_step32(const OptStep& h, T* p, const float g
     pv[j] = pv[j] * h.decay - h.rate * opt_update(mv[j], vv[j], h.root, h.eps);
   }
   opt_store4<WHOLE>(p, i, n, pv);
-  opt_store4<WHOLE>(m, i, n, mv);
-  opt_store4<WHOLE>(v, i, n, vv);
+  opt_store4<WHOLE, true>(m, i, n, mv);
+  opt_store4<WHOLE, true>(v, i, n, vv);
 }

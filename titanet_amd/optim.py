@@ -167,15 +167,7 @@ class AdamW(torch.optim.Optimizer):
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters as flat float32 tensors: parameter i's from ``BLOCK * first`` on, every
         parameter at a multiple of 256, zeros between them.  32 bits: the buffers themselves; 8 bits: the values of the codes."""
-        if self.state_bits == 32 or self._device is None:
-            return self._exp_avg, self._exp_avg_sq
-        with torch.cuda.device(self._device):
-            m = torch.empty(self.blocks * BLOCK, dtype=torch.float32, device=self._device)
-            v = torch.empty_like(m)
-            check(self._native.tn_moments_decode(_dev(self._exp_avg), _dev(self._exp_avg_sq), _dev(self._scale1), _dev(self._scale2), _dev(m),
-                                                 _dev(v), self.blocks, C.c_void_p(torch.cuda.current_stream(self._device).cuda_stream)),
-                  "tn_moments_decode")
-        return m, v
+        return self._stepper.moments() if self._device is not None else (self._exp_avg, self._exp_avg_sq)
 
     @torch.no_grad()
     def load_moments(self, exp_avg, exp_avg_sq, step):
