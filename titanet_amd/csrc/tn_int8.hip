@@ -282,6 +282,7 @@ __device__ __forceinline__ i32x4_t q8_srd(const void* base, int64_t bytes) {
   r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(b >> 32) & 0xffffu));
   r[2] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(bytes < 0x7fffffff ? (bytes > 0 ? bytes : 0) : 0x7fffffff));
   r[3] = 0x00020000;
+  asm volatile("s_nop 4" : "+s"(r));                // (a descriptor written by the vector unit is not for the next five states' memory access)
   return r;
 }
 // 64 lanes x 16 bytes from descriptor + voff + soff into LDS at lds_addr + 16 * lane; zeros from the descriptor's end on.  The
@@ -305,68 +306,83 @@ __device__ __forceinline__ void q8_barrier_after_reads() {
   q8_barrier();
 }
 
+// Workgroup b runs on XCD b % 8: each XCD takes a run of neighbouring tiles, so that the tiles of one row of tiles read their common
+// operand rows through one L2.
+__device__ __forceinline__ int q8_tile(int tiles) {
+  const int per = tiles / 8, more = tiles % 8, xcd = blockIdx.x % 8;
+  return xcd * per + (xcd < more ? xcd : more) + blockIdx.x / 8;
+}
+
 template <typename T>
 struct Q8Pair {
   typedef T type __attribute__((ext_vector_type(2), aligned(sizeof(T))));
 };
-
-// TM x TN outputs per workgroup of 4 waves (2 x 2), operands through LDS in steps of 128 bytes of K, NS steps in flight.  LDS image:
-// rows of 128 bytes, chunk of 16 bytes ^= row & 7 (applied to the source address of the LDS-DMA, undone by the fragment reads:
-// eight rows of one chunk fall into eight different bank groups).  Weight row 2 i + j of a wave's 64-column block lies at image row
-// 32 j + i: a lane then owns two neighbouring columns and stores them together.
-template <typename Y, int TM, int TN, int NS>
-__global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n) {
-  constexpr int STEP = 128, STAGE = (TM + TN) * STEP, QA = TM / 32, QB = TN / 32;      // DMA instructions per wave and operand
+// TM x TN outputs per workgroup of 4 waves (2 x 2), operands through LDS in steps of STEP bytes of K, NS steps in flight, one tile to
+// a workgroup: its stores drain while the next one on the compute unit multiplies (a persistent workgroup would wait for them with
+// its next operands: loads and stores return in one order).  LDS image: rows of STEP bytes, chunk of 16 bytes ^= row / 2 & 7 (128) or
+// row / 4 & 3 (64), applied to the source address of the LDS-DMA and undone by the fragment reads: sixteen rows of one chunk fall into
+// sixteen different groups of the 64 banks.  Weight row 2 i + j of a wave's 64-column block lies at image row 32 j + i: a lane then owns
+// two neighbouring columns and stores them together.
+// Bound by stores for short sums (4708 x 50021 x 192 to float32: 226 us, 4.2 TB/s) and for long ones by the matrix pipe at the clock
+// that the chip's power leaves it: 2.9 POP/s fed from registers alone; 76800 x 1536 x 1536 in 290 us, where the library's product to
+// 32-bit integers takes 268, 76800 x 1024 x 1024 in 132 (148), 76800 x 512 x 512 in 41 - 48 (56), 2048 x 2048 x 2048 in 17 (21).  Built and
+// not kept: tiles of 256 x 256 by 8 waves, persistent with LDS-DMA (267 us) or one to a workgroup through registers, one or two steps
+// ahead (272 - 308, 288), 128 x 256 and 256 x 128 by 4 waves (278 - 297): within a tenth on the largest shape, behind on the others.
+template <typename Y, int TM, int TN, int STEP, int NS>
+__global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles_m, int tiles_n, bool down) {
+  constexpr int STAGE = (TM + TN) * STEP, CPR = STEP / 16, RP = 64 / CPR, SH = STEP == 128 ? 1 : 2;
+  constexpr int QA = TM / (4 * RP), QB = TN / (4 * RP);      // DMA instructions per wave and operand, RP rows each
   constexpr int WM = TM / 2, WN = TN / 2, MI = WM / 32, NJ = WN / 64;
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   const unsigned lds0 = (unsigned)(uintptr_t)(q8_lds_char*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
   const int fi = lane & 31, fh = lane >> 5;
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * TM, n0 = (int64_t)(blockIdx.x % tiles_n) * TN;
+  const int tile = q8_tile(gridDim.x);
+  const int64_t m0 = (int64_t)(down ? tile % tiles_m : tile / tiles_n) * TM, n0 = (int64_t)(down ? tile / tiles_m : tile % tiles_n) * TN;
   const int64_t rows_a = g.m - m0 < TM ? g.m - m0 : TM, rows_b = g.n - n0 < TN ? g.n - n0 : TN;
   const i32x4_t sa = q8_srd(g.a + m0 * g.lda, rows_a * g.lda), sb = q8_srd(g.b + n0 * g.ldb, rows_b * g.ldb);
   const int tr = (int)(threadIdx.x < rows_a ? threadIdx.x : rows_a - 1), tc = (int)(threadIdx.x < rows_b ? threadIdx.x : rows_b - 1);
   const float in_sa = g.sa[m0 + tr], in_sb = g.sb[n0 + tc], in_bias = g.bias ? g.bias[n0 + tc] : 0.f;
-  const int chunk = (lane & 7) ^ (lane >> 3);
+  const int chunk = (lane % CPR) ^ (((wave * RP + lane / CPR) >> SH) & (CPR - 1));      // (4 * RP rows further the same)
   unsigned offa[QA], offb[QB];
 #pragma unroll
-  for (int q = 0; q < QA; ++q) offa[q] = (unsigned)((q * 4 + wave) * 8 + (lane >> 3)) * (unsigned)g.lda + chunk * 16;
+  for (int q = 0; q < QA; ++q) offa[q] = (unsigned)((q * 4 + wave) * RP + lane / CPR) * (unsigned)g.lda + chunk * 16;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    const int p = (q * 4 + wave) * 8 + (lane >> 3);
+    const int p = (q * 4 + wave) * RP + lane / CPR;
     offb[q] = (unsigned)((p & ~63) + 2 * (p & 31) + ((p >> 5) & 1)) * (unsigned)g.ldb + chunk * 16;
   }
   const int steps = (g.k + STEP - 1) / STEP;
-  auto request = [&](int t) {
+  auto request = [&](int t, int stage) {
     if (t >= steps) return;
-    const unsigned at = lds0 + (t % NS) * STAGE, soff = t * STEP;
-    const bool in = t * STEP + chunk * 16 < g.k;
+    const unsigned at = lds0 + stage * STAGE, soff = t * STEP, none = t * STEP + chunk * 16 < g.k ? 0u : 0x80000000u;
 #pragma unroll
-    for (int q = 0; q < QA; ++q) q8_dma(in ? offa[q] : 0x80000000u, sa, soff, __builtin_amdgcn_readfirstlane(at + (q * 4 + wave) * 1024));
+    for (int q = 0; q < QA; ++q) q8_dma(offa[q] | none, sa, soff, __builtin_amdgcn_readfirstlane(at + (q * 4 + wave) * 1024));
 #pragma unroll
-    for (int q = 0; q < QB; ++q) q8_dma(in ? offb[q] : 0x80000000u, sb, soff, __builtin_amdgcn_readfirstlane(at + TM * STEP + (q * 4 + wave) * 1024));
+    for (int q = 0; q < QB; ++q) q8_dma(offb[q] | none, sb, soff, __builtin_amdgcn_readfirstlane(at + TM * STEP + (q * 4 + wave) * 1024));
   };
   i32x16_t acc[MI][NJ][2] = {};
 #pragma unroll
-  for (int t = 0; t < NS; ++t) request(t);
-  int foff[4];
+  for (int t = 0; t < NS; ++t) request(t, t);
+  int foff[STEP / 32];
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) foff[ks] = fi * STEP + (((2 * ks + fh) ^ (fi & 7)) << 4);
+  for (int ks = 0; ks < STEP / 32; ++ks) foff[ks] = fi * STEP + (((2 * ks + fh) ^ ((fi >> SH) & (CPR - 1))) << 4);
+  int stage = 0;
   for (int t = 0; t < steps; ++t) {
     if (t + NS <= steps) q8_wait<(NS - 1) * (QA + QB)>();      // step t has landed; the later ones stay in flight
     else q8_wait<0>();
     q8_barrier();
-    const int8_t* st = smem + (t % NS) * STAGE;
+    const int8_t* st = smem + stage * STAGE;
     const int8_t *pa = st + wm * WM * STEP, *pb = st + TM * STEP + wn * WN * STEP;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < STEP / 32; ++ks) {
       i32x4_t af[MI], bf[NJ][2];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(pa + i * 32 * STEP + foff[ks]);
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) bf[j][h] = *reinterpret_cast<const i32x4_t*>(pb + (j * 64 + h * 32) * STEP + foff[ks]);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(pa + i * 32 * STEP + foff[ks]);
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -375,7 +391,8 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args g, int tiles_n)
           for (int h = 0; h < 2; ++h) acc[i][j][h] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[i], bf[j][h], acc[i][j][h], 0, 0, 0);
     }
     q8_barrier_after_reads();                       // everybody has read this stage
-    request(t + NS);
+    request(t + NS, stage);
+    stage = stage + 1 == NS ? 0 : stage + 1;
   }
   // ---- epilogue: scales and bias of the tile through LDS (a load per output row would be waited for row by row)
   float* sc = reinterpret_cast<float*>(smem);       // [TM] token scales, [TN] channel scales, [TN] bias
@@ -462,13 +479,19 @@ int q8_few_rows(const FewArgs& f, void* stream) {
 
 template <typename Y>
 int q8_tiles(const Int8Args& g, void* stream) {
-  auto go = [&](auto tm, auto tn, auto ns) -> int {
-    constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, NS = decltype(ns)::value;
-    const int64_t a = (g.m + TM - 1) / TM, b = (g.n + TN - 1) / TN;
+  auto go = [&](auto step, bool down) -> int {
+    constexpr int T = 128, STEP = decltype(step)::value, NS = 2;
+    const int64_t a = (g.m + T - 1) / T, b = (g.n + T - 1) / T;
     if (b > Q8_GRID || a > Q8_GRID / b) return TN_E_UNSUPPORTED;
-    return q8_launch(int8_tile_kernel<Y, TM, TN, NS>, dim3((unsigned)(a * b)), 256, (size_t)NS * (TM + TN) * 128, stream, g, (int)b);
+    return q8_launch(int8_tile_kernel<Y, T, T, STEP, NS>, dim3((unsigned)(a * b)), 256, (size_t)NS * 2 * T * STEP, stream, g, (int)a, (int)b, down);
   };
-  return go(std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
+  // Up to 8 rows of tiles one after another share a column of weights (read once) before the next column; with more of them the
+  // tiles run along the rows.  Rows / columns first: 250 x 100003 x 192 36.5 / 30.0 us, 1000 x 50000 x 192 52 / 41, but 4708 x 50021 x
+  // 192 173 / 214 and 76800 x 1536 x 1536 291 / 314 (bf16 outputs).  Short sums of few rows are bound by their stores: steps of 64 bytes
+  // leave room for twice the workgroups (250 x 100003 x 192 21.3 us, 1000 x 50000 x 192 30.1); everything else takes whole lines of
+  // 128 (4708 x 50021 x 192 173 against 199 us, 76800 x 1536 x 1536 291 against 328, 2048 x 2048 x 2048 17 against 19).
+  const bool down = g.m <= 8 * 128;
+  return down && g.k <= 512 ? go(std::integral_constant<int, 64>{}, down) : go(std::integral_constant<int, 128>{}, down);
 }
 
 bool q8_operands_ok(int64_t m, int64_t n, int64_t k, const void* b, const float* b_scales, int64_t ldb, const void* y, int64_t ldy) {
