@@ -20,12 +20,11 @@ HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".h")) + ["../../incl
 OUT = os.path.join(PKG, "libtitanet_amd.so")
 HOST_SOURCE, HOST_OUT = "tn_host.cpp", os.path.join(PKG, "_host.so")      # Python module over torch tensors, linked to the library
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
-         "-Wno-unused-variable"]
+         "-Wno-unused-variable",
+         # ordinary float code becomes packed single-precision instructions at -O3 unless told otherwise; some of their forms are not
+         # to be relied on, so no kernel here uses them (hipcc's host pass warns that it does not know the feature: harmless)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-
-# ordinary float code becomes packed single-precision instructions at -O3 unless told otherwise; some of their forms are not to be
-# relied on, so no kernel here uses them
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _digest():
@@ -63,7 +62,7 @@ def build(force=False, verbose=True):
 
     def cc(src):
         obj = os.path.join(HERE, src.replace(".hip", ".o"))
-        cmd = [hipcc] + FLAGS + (NO_PACKED_FP32 if src in SOURCES[3:] else []) + ["-c", os.path.join(HERE, src), "-o", obj]
+        cmd = [hipcc] + FLAGS + ["-c", os.path.join(HERE, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
