@@ -299,6 +299,39 @@ def test_a_captured_step_replays(bits):
             frozen.step()
 
 
+def test_a_partial_step_is_not_captured_and_two_graphs_share_an_optimizer():
+    """a graph for each of two gradient buffers, replayed in turn with eager steps between them"""
+    p, q = _tensors([5000], torch.float32, 25)[0], _tensors([5000], torch.float32, 25)[0]
+    lr, lr2 = (torch.full((), 1e-2, device="cuda") for _ in range(2))
+    opt, eager = AdamW([p], lr=lr, max_grad_norm=1.0, state_bits=8), AdamW([q], lr=lr2, max_grad_norm=1.0, state_bits=8)
+    grads, graphs = _grads([5000, 5000], torch.float32, 26), []
+    p.grad = grads[0]
+    opt.step()
+    q.grad = grads[0]
+    eager.step()
+    for g in grads:
+        p.grad = g
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            opt.step()
+    for k in (0, 1, 1, 0, 2, 0, 1):
+        if k < 2:
+            graphs[k].replay()
+            q.grad = grads[k]
+        else:
+            p.grad = q.grad = grads[0] * 0.5
+            opt.step()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(opt.moments(), eager.moments())), k
+    a, b = (torch.ones(300, device="cuda") for _ in range(2))
+    some = AdamW([a, b], lr=lr)
+    a.grad = torch.ones(300, device="cuda")
+    with pytest.raises(RuntimeError, match="run such a step once"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            some.step()
+
+
 def test_on_another_stream():
     params, twin = _tensors([100000], torch.float32, 21), _tensors([100000], torch.float32, 21)
     opt, plain = AdamW(params, max_grad_norm=0.1), AdamW(twin, max_grad_norm=0.1)
@@ -353,6 +386,13 @@ def test_checkpoints_of_either_width_and_torchs():
     other.load_moments(m, v, step=3)
     for a, b in zip((other._exp_avg, other._exp_avg_sq, other._scale1, other._scale2), (narrow._exp_avg, narrow._exp_avg_sq, narrow._scale1, narrow._scale2)):
         assert torch.equal(a, b)
+    # a tensor lr stays the tensor it is (a captured step reads it) and takes the loaded value
+    lr = torch.full((), 5.0, device="cuda")
+    held = AdamW([p.clone() for p in params], lr=lr, state_bits=8)
+    held.load_state_dict(codes)
+    assert held.param_groups[0]["lr"] is lr and abs(float(lr) - 1e-2) < 1e-9
+    with pytest.raises(TypeError, match="state_dict"):
+        copy.deepcopy(other)
     with pytest.raises(ValueError):
         other.load_moments(m[1:], v[1:], step=1)
     with pytest.raises(ValueError):

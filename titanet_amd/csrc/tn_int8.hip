@@ -34,9 +34,18 @@ __device__ __forceinline__ int q8_code(float x, float s, float inv) {
 
 __device__ __forceinline__ float q8_scale(float top) { return top > 0.f ? fmaxf(top / 127.f, 0x1p-126f) : 0.f; }
 
-__device__ __forceinline__ float q8_max_group(float x, int group) {       // over aligned groups of `group` lanes
-  for (int d = group >> 1; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
-  return x;
+// largest of an aligned group of GROUP lanes' numbers (none negative, so their bit patterns are ordered like them)
+template <int GROUP>
+__device__ __forceinline__ float q8_max_group(float f) {
+  int x = __float_as_int(f);
+  auto up = [&](int y) { x = x > y ? x : y; };
+  up(__builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false));                       // lane ^ 1
+  up(__builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, false));                       // lane ^ 2
+  up(__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false));                      // mirrored within 8
+  if (GROUP >= 16) up(__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, false));     // mirrored within 16
+  if (GROUP >= 32) up(__shfl_xor(x, 16, 64));
+  if (GROUP >= 64) up(__shfl_xor(x, 32, 64));
+  return __int_as_float(x);
 }
 
 // eight consecutive elements from k on as floats, zeros behind the row's end; the type's own alignment is enough
@@ -55,7 +64,7 @@ __device__ __forceinline__ void q8_load8(const T* row, int k, int cols, float v[
     for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? (float)row[k + j] : 0.f;
   }
 }
-// largest |v|, NaN where one of them is not finite (a later maximum then has to look for it: fmaxf drops NaN)
+// largest |v|; bad where one of them is not finite (a maximum drops NaN)
 __device__ __forceinline__ float q8_top8(const float v[8], float top, bool& bad) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
@@ -112,7 +121,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
         top = q8_top8(v[0], top, bad);
       }
     }
-    top = q8_max_group(bad ? __builtin_huge_valf() : top, GROUP);
+    top = q8_max_group<GROUP>(bad ? __builtin_huge_valf() : top);
     const bool finite = top < __builtin_huge_valf();
     const float s = finite ? q8_scale(top) : 0.f, inv = s > 0.f ? 1.f / s : 0.f;
     uint2* out = reinterpret_cast<uint2*>(q + r * ldq);
@@ -157,7 +166,7 @@ struct FewArgs {
 
 template <typename X, typename Y, int NW, int KS>
 __global__ __launch_bounds__(NW * 64) void int8_few_rows_kernel(FewArgs f) {
-  constexpr int G = NW / KS, AHEAD = 6;
+  constexpr int G = NW / KS, AHEAD = KS == 16 ? 3 : 6;      // weight loads on their way before the rows' codes are made
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   const Int8Args& g = f.g;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fi = lane & 31, fh = lane >> 5;
@@ -203,7 +212,7 @@ __global__ __launch_bounds__(NW * 64) void int8_few_rows_kernel(FewArgs f) {
         q8_load8(row, k, f.cols, w);
         top = q8_top8(w, top, bad);
       }
-      top = q8_max_group(bad ? __builtin_huge_valf() : top, 64);
+      top = q8_max_group<64>(bad ? __builtin_huge_valf() : top);
       const bool finite = top < __builtin_huge_valf();
       const float s = finite ? q8_scale(top) : 0.f, inv = s > 0.f ? 1.f / s : 0.f;
       uint2* out = reinterpret_cast<uint2*>(smem + r * pitch);

@@ -437,7 +437,7 @@ extern "C" int tn_adamw_tick(int32_t count, const int32_t* slots, const tn_adamw
   for (int i = 0; i < count; ++i)
     if (slots[i] < 0) return TN_E_BADARG;
   const NormArgs a = {partials, n_partials, grad_mult, max_norm, norm, ctl};
-  for (int lo = 0; lo < count; lo += 256) {
+  for (int lo = 0; lo < count || (partials && lo == 0); lo += 256) {      // (without slots the norm still ends)
     OptSlots list;
     list.count = std::min(256, count - lo);
     for (int i = 0; i < list.count; ++i) list.slot[i] = slots[lo + i];

@@ -66,6 +66,9 @@ class AdamW(torch.optim.Optimizer):
         self.blocks = 0
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        raise TypeError("AdamW holds device buffers laid out for its parameters: save state_dict() instead of pickling or copying it")
+
     # ------------------------------------------------------------------ layout
     def add_param_group(self, param_group):
         params = param_group["params"]
@@ -253,8 +256,10 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("loaded state dict is of a variant (amsgrad, maximize) that AdamW does not have")
             hyper = {k: v for k, v in g.items() if k in ("lr", "betas", "eps", "weight_decay")}
             self._check_hyper({**o, **hyper})
-            if isinstance(hyper.get("lr"), torch.Tensor) and self._device is not None:
-                hyper["lr"] = hyper["lr"].to(self._device).clone()
+            if "lr" in hyper and isinstance(o["lr"], torch.Tensor):
+                o["lr"].fill_(hyper.pop("lr"))               # (a captured step reads this tensor)
+            elif isinstance(hyper.get("lr"), torch.Tensor):
+                hyper["lr"] = hyper["lr"].to(self._device or hyper["lr"].device).clone()
             o.update({**{k: v for k, v in g.items() if k not in ("params", "lr", "betas", "eps", "weight_decay")}, **hyper})
         if self._device is None:
             return
