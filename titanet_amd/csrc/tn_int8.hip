@@ -97,8 +97,8 @@ __device__ __forceinline__ uint2 q8_pack8(const float v[8], float s, float inv) 
 }
 
 // Codes and scale of every row.  A row belongs to GROUP lanes of a wave, eight elements to a lane and pass, kept in registers
-// between the maximum and the codes where PASSES of them hold the row (PASSES = 0: read twice).  One pass over memory; what
-// bounds it is HBM.
+// between the maximum and the codes where PASSES of them hold the row (PASSES = 0: read twice).  One pass over memory and bound by
+// it: 76800 x 1536 bfloat16 in 78 - 90 us, 3.9 - 4.5 TB/s (258 us element by element, 97 with 20 instructions a value).
 template <typename T, int GROUP, int PASSES>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ q,
                                                             int64_t ldq, int padded, float* __restrict__ scales) {
@@ -156,7 +156,8 @@ __device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) { r
 // The weight is read once, straight from memory into matrix operands (a lane's 16 bytes of one weight row); the rows' codes are
 // made by every workgroup for itself in LDS while the first weight loads are on their way, so one launch does it all.  NW waves
 // share a tile of 32 channels by splitting K in KS parts (joined through LDS: integer sums, any order gives the same) or work on
-// NW / KS tiles.  Bound by the latency of load - maximum - codes - product for small weights, by HBM for large ones.
+// NW / KS tiles.  Bound by the latency of load - maximum - codes - product for small weights (1 x 7205 x 192 4.6 us, 16 x 192 x 1536 from
+// float 6.3 us; quantised by a launch of its own and multiplied in tiles they took 8.4 and 28), by HBM for large ones.
 struct FewArgs {
   const void* x;                      // rows of X, or codes with scales sa
   Int8Args g;
