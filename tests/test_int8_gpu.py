@@ -115,6 +115,14 @@ def test_strides_shapes_and_empty_operands():
     assert torch.equal(int8_matmul(x[3:4, 8:104].expand(5, 96), w), plain[3:4].expand(5, 40))
     assert torch.equal(int8_matmul(x[::3, 8:104], w), plain[::3])
     assert int8_matmul(x[:0, 8:104], w).shape == (0, 40) and int8_matmul(x[:, :5], quantize_rows(x[:0, :5])).shape == (24, 0)
+    for t in (torch.bfloat16, torch.float16, torch.float32):                                      # rows that begin at any element
+        odd = x.to(t).view(-1)[1:24 * 199 + 1].view(24, 199)
+        for first in (1, 2, 5):
+            for m in (3, 24):
+                part = odd[:m, first:first + 96]
+                assert torch.equal(int8_matmul(part, w), int8_matmul(part.contiguous(), w)) and torch.equal(quantize_rows(part).codes, quantize_rows(part.contiguous()).codes)
+        tall = x.to(t).repeat(3, 1)[:, 3:99]
+        assert torch.equal(int8_matmul(tall, w), int8_matmul(tall.contiguous(), w))
     inner = torch.zeros(40, 200, dtype=torch.int8, device="cuda")
     inner[:, 3:99] = w.codes
     inner[:, 99:] = 77                                                                            # what lies behind the codes is no part of them
