@@ -495,3 +495,28 @@ def test_titanet_parameters(bits):
             # the first step does not depend on how moments are held, but for the roundings of 32 bits
             torch.testing.assert_close(flat, model.flat_parameters(), rtol=6 * U, atol=1e-3 * 32 * U)
     assert bool(torch.isfinite(model.flat_parameters()).all())
+
+
+@pytest.mark.parametrize("top", [3e38, 2.0 ** 127, 1.7e38, 2.0 ** 126, 2.0 ** 125, 1e30, 2.0 ** -99, 2.0 ** -100, 2.0 ** -101, 1e-31, 1e-37, 1e-40, 2.0 ** -149])
+def test_codes_of_the_largest_and_smallest_scales(top):
+    """blocks whose largest moment lies near either end of float32: codes and scales are the definition's"""
+    top = float(np.float32(top))
+    x = torch.randn(700, generator=torch.Generator().manual_seed(35), dtype=torch.float64)
+    x = (x / x.abs().max() * top).float()
+    x[[0, 256]], x[699] = top, -top
+    m, v = (torch.zeros(768, device="cuda") for _ in range(2))
+    m[:700], v[:700] = x.cuda(), x.abs().cuda()
+    opt = AdamW([torch.zeros(700, device="cuda")], state_bits=8)
+    opt.load_moments(m, v, step=5)
+    for codes, scales, back, y, second in zip((opt._exp_avg, opt._exp_avg_sq), (opt._scale1, opt._scale2), opt.moments(), (x, x.abs()), (False, True)):
+        want, tops = O.encode(y.double().numpy(), second)
+        assert np.array_equal(scales.cpu().numpy(), tops) and np.array_equal(codes[:700].cpu().numpy().astype(np.int64), want)
+        np.testing.assert_allclose(back[:700].cpu().numpy(), O.decode(want, tops, second), rtol=4 * U, atol=1.5e-45)
+
+
+def test_8_bit_steps_whose_squares_come_near_the_largest_float():
+    params = _tensors([700], torch.float32, 3)
+    opt, o = AdamW(params, state_bits=8), O.Tensor(_np(params[0]), 8)
+    for scale in (1.2e20, 1e19, 0.0):
+        _follow(opt, params, [o], "fp32", 8, [scale * _tensors([700], torch.float32, 4)[0]], lr=1e-3)
+        assert scale < 1e20 or 2.0 ** 126 < float(opt._scale2.max()) < float("inf")

@@ -127,9 +127,10 @@ __device__ __forceinline__ float opt_scale_wave(const float f[4]) {
   top = opt_max_wave(top);
   return top < 0x7f800000u ? __uint_as_float(top) : __builtin_nanf("");
 }
-// x / scale to float accuracy, for candidates; a scale whose reciprocal a float cannot hold goes through 64 bits
+// x / scale to float accuracy, for candidates; a scale whose reciprocal a float cannot hold goes through 64 bits: below 2^-100, and from
+// 2^125 on, since the hardware's reciprocal has no denormal results (1 / 2^127 is 0, and every code of the block would be 1 at most)
 __device__ __forceinline__ void opt_ratio(const double x[4], const float f[4], float scale, float r[4]) {
-  if (scale > 0x1p-100f) {             // (uniform over the wave)
+  if (scale > 0x1p-100f && scale < 0x1p125f) {             // (uniform over the wave)
     const float inv = __builtin_amdgcn_rcpf(scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = fabsf(f[j]) * inv;
