@@ -238,3 +238,28 @@ def test_every_output_of_large_products_time_after_time(m, n, k):
     qa, qb = Int8Rows(a, sa), Int8Rows(b, sb)
     for _ in range(6):
         assert torch.equal(int8_matmul(qa, qb), want)
+
+
+@pytest.mark.parametrize("m", [1, 5, 32, 33, 200])
+@pytest.mark.parametrize("n,k", [(7, 64), (130, 192), (251, 700)])
+def test_large_rows_against_small_weights(m, n, k):
+    """rows whose sums times one scale leave float32 while the products do not, ordinary and tiny rows beside them"""
+    x, w = _x(m, k, 30), _x(n, k, 31) * 1e-4
+    x[::3] *= 3e37 / float(x.abs().max())
+    x[1::3] *= 1e-30
+    x[2::6] = 0
+    for a, b, out in ((x, w, "fp32"), (x, w, "bf16"), (w, x, "fp32")):
+        want, part = O.product(*O.quantize(_np(a)), *O.quantize(_np(b)))
+        assert np.abs(want).max() < 3e38
+        for left in (a, quantize_rows(a)):
+            _compare(int8_matmul(left, quantize_rows(b), out_dtype={"fp32": torch.float32, "bf16": torch.bfloat16}[out]), want, part, out)
+
+
+@pytest.mark.parametrize("m,k", [(31, 192), (32, 1), (32, 192), (32, 1984), (32, 1985), (31, 2048), (31, 2049)])
+def test_products_at_the_ends_of_the_few_rows_kernel(m, k):
+    """the most rows, and the longest for that many, that are quantised inside the product, and the next ones"""
+    for n in (5, 130):
+        x, w = _x(m, k, 32), _x(n, k, 33)
+        want, part = O.product(*O.quantize(_np(x)), *O.quantize(_np(w)))
+        for a in (x, quantize_rows(x)):
+            _compare(int8_matmul(a, quantize_rows(w)), want, part, "fp32")

@@ -149,8 +149,16 @@ struct Int8Args {
   int k;                              // multiple of 64
 };
 
-template <typename T>
-__device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) { return (T)((float)acc * sa * sb + bias); }
+// The sum times both scales.  The sum is a whole number below 2^32, so times a token scale below 2^96 it stays in range (and a small scale
+// costs nothing: the product is a multiple of the scale's own last place).  A larger token scale (rows from 1e31 on) goes last: the sum
+// times it could leave 32 bits where the product does not.
+constexpr float Q8_FAR = 0x1p96f;
+template <typename T, bool FAR>
+__device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) {
+  if constexpr (!FAR) return (T)((float)acc * sa * sb + bias);
+  const bool last = sa >= Q8_FAR;
+  return (T)((float)acc * (last ? sb : sa) * (last ? sa : sb) + bias);
+}
 
 // ------------------------------------------------------------------------------------------------------- few rows (m <= 32)
 // The weight is read once, straight from memory into matrix operands (a lane's 16 bytes of one weight row); the rows' codes are
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(NW * 64) void int8_few_rows_kernel(FewArgs f) {
   auto store = [&](int64_t t, int r, int sum, float sb, float bias) {
     const int row = (r & 3) + 8 * (r >> 2) + 4 * fh;
     const int64_t col = t * 32 + fi;
-    if (row < m && col < g.n) y[row * g.ldy + col] = q8_out<Y>(sum, scales[row], sb, bias);
+    if (row < m && col < g.n) y[row * g.ldy + col] = q8_out<Y, true>(sum, scales[row], sb, bias);
   };
   bool held = true;
   for (int64_t base = (int64_t)blockIdx.x * G; base < tiles; base += stride, tile += stride) {      // uniform over the workgroup
@@ -405,15 +413,18 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles
     stage = stage + 1 == NS ? 0 : stage + 1;
   }
   // ---- epilogue: scales and bias of the tile through LDS (a load per output row would be waited for row by row)
-  float* sc = reinterpret_cast<float*>(smem);       // [TM] token scales, [TN] channel scales, [TN] bias
+  float* sc = reinterpret_cast<float*>(smem);       // [TM] token scales, [TN] channel scales, [TN] bias, a wave's word each: a far token scale
+  static_assert(TM <= 128 && (TM + 2 * TN + 2) * 4 <= STAGE, "token scales come from the first two waves");
   if (threadIdx.x < TM) sc[threadIdx.x] = in_sa;
+  if (threadIdx.x < 128) sc[TM + 2 * TN + wave] = __ballot(in_sa >= Q8_FAR) ? 1.f : 0.f;
   if (threadIdx.x < TN) {
     sc[TM + threadIdx.x] = in_sb;
     sc[TM + TN + threadIdx.x] = in_bias;
   }
   __syncthreads();
+  const bool far = sc[TM + 2 * TN] + sc[TM + 2 * TN + 1] != 0.f;
   Y* y = reinterpret_cast<Y*>(g.y);
-  auto put = [&](auto whole) {
+  auto put = [&](auto whole, auto far) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int c = wn * WN + j * 64 + 2 * fi;
@@ -429,7 +440,7 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles
           const int64_t row = m0 + rw;
           if (!whole && row >= g.m) continue;
           const float s = sc[rw];
-          const Y y0 = q8_out<Y>(acc[i][j][0][r], s, s0, b0), y1 = q8_out<Y>(acc[i][j][1][r], s, s1, b1);
+          const Y y0 = q8_out<Y, far>(acc[i][j][0][r], s, s0, b0), y1 = q8_out<Y, far>(acc[i][j][1][r], s, s1, b1);
           if (two) {
             typename Q8Pair<Y>::type v;
             v[0] = y0;
@@ -441,8 +452,9 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles
         }
     }
   };
-  if (rows_a == TM && rows_b == TN) put(std::true_type{});
-  else put(std::false_type{});
+  if (far) put(std::false_type{}, std::true_type{});
+  else if (rows_a == TM && rows_b == TN) put(std::true_type{}, std::false_type{});
+  else put(std::false_type{}, std::false_type{});
 }
 
 template <typename F>
