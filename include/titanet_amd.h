@@ -220,8 +220,10 @@ typedef struct tn_adamw_state { /* device memory */
   int64_t blocks;               /* how many blocks of 256 the moment buffers hold */
   void *exp_avg, *exp_avg_sq;   /* float, or int8 and uint8 */
   float *scale1, *scale2;       /* 8 bits: [blocks] */
-  int32_t* steps;               /* by slot: tensors that have always been stepped together share one */
+  int32_t* steps;               /* by slot: how often the tensors that name it have been stepped */
   float* corr;                  /* float[4] by slot, 16-byte aligned: what the step derives from the count */
+  const int32_t* owner;         /* NULL, or by block the slot of its tensor, read by the kernels instead of the lists' slots: what a
+                                   captured step needs whose tensors come to different counts between replays */
 } tn_adamw_state;
 typedef struct tn_adamw_lists { /* tensors of one type */
   int32_t count, dtype;

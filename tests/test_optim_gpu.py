@@ -520,3 +520,75 @@ def test_8_bit_steps_whose_squares_come_near_the_largest_float():
     for scale in (1.2e20, 1e19, 0.0):
         _follow(opt, params, [o], "fp32", 8, [scale * _tensors([700], torch.float32, 4)[0]], lr=1e-3)
         assert scale < 1e20 or 2.0 ** 126 < float(opt._scale2.max()) < float("inf")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_and_steps_of_some_tensors_count_together(bits):
+    """replays, eager steps of all or of some tensors and loaded states, in any order: every tensor has its own count"""
+    sizes = [256, 512, 300, 64]                  # the first ones follow one another in memory, whole blocks
+    values, grads = torch.cat(_tensors(sizes, torch.float32, 36)), torch.cat(_grads(sizes, torch.float32, 37))
+
+    def build():
+        params, at = list(values.clone().split(sizes)), list(grads.clone().split(sizes))
+        return params, at, AdamW(params, lr=torch.full((), 1e-2, device="cuda"), state_bits=bits, max_grad_norm=0.3)
+    (p, g, opt), (q, h, eager) = build(), build()
+
+    def give(active):
+        for k in range(4):
+            p[k].grad, q[k].grad = (g[k], h[k]) if k in active else (None, None)
+
+    def same(what):
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(p, q)), what
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(), eager.moments())), what
+        a, b = ({i: int(e["step"]) for i, e in o.state_dict()["state"].items()} for o in (opt, eager))
+        assert a == b, (what, a, b)
+
+    def some(*active):
+        give(active)
+        opt.step()
+        eager.step()
+        same(("eager", active))
+
+    def replay(graph):
+        graph.replay()
+        give(range(4))
+        eager.step()
+        same("replay")
+
+    def capture():
+        give(range(4))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        return graph
+
+    some(0, 1, 2, 3)
+    first = capture()
+    replay(first)
+    for _ in range(3):
+        some(0)
+    replay(first)
+    some(1, 3)
+    second = capture()
+    for graph in (second, first, second):
+        replay(graph)
+        some(0, 1, 2, 3)
+    state = copy.deepcopy(eager.state_dict())
+    unequal = copy.deepcopy(state)
+    for e in state["state"].values():
+        e["step"] = torch.tensor(7.0)
+    for loaded in (state, unequal, state):
+        opt.load_state_dict(copy.deepcopy(loaded))
+        eager.load_state_dict(copy.deepcopy(loaded))
+        for graph in (first, second):
+            replay(graph)
+            some(2)
+            some(0, 1, 2, 3)
+    m, v = (x.clone() for x in eager.moments())
+    for o in (opt, eager):
+        o.load_moments(m, v, step=2)
+    replay(second)
+    some(1)
+    replay(first)
+    some(0, 1, 2, 3)

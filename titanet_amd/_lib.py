@@ -43,7 +43,7 @@ class TnAdamwHyper(C.Structure):
 
 class TnAdamwState(C.Structure):
     _fields_ = [("bits", C.c_int32), ("blocks", C.c_int64), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("scale1", C.c_void_p),
-                ("scale2", C.c_void_p), ("steps", C.c_void_p), ("corr", C.c_void_p)]
+                ("scale2", C.c_void_p), ("steps", C.c_void_p), ("corr", C.c_void_p), ("owner", C.c_void_p)]
 
 
 class TnAdamwLists(C.Structure):

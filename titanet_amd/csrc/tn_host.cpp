@@ -77,8 +77,8 @@ class Stepper {
  public:
   Stepper(int bits) : bits_(bits) {}
 
-  void layout(std::vector<int64_t> numel, std::vector<int64_t> first, std::vector<int32_t> slots, int64_t blocks, at::Tensor exp_avg,
-              at::Tensor exp_avg_sq, std::optional<at::Tensor> scale1, std::optional<at::Tensor> scale2, at::Tensor steps, at::Tensor corr) {
+  void layout(std::vector<int64_t> numel, std::vector<int64_t> first, std::vector<int32_t> sets, int64_t blocks, at::Tensor exp_avg,
+              at::Tensor exp_avg_sq, std::optional<at::Tensor> scale1, std::optional<at::Tensor> scale2, at::Tensor steps, at::Tensor corr, at::Tensor owner) {
     numel_ = std::move(numel);
     first_ = std::move(first);
     blocks_ = blocks;
@@ -88,13 +88,15 @@ class Stepper {
     scale2_ = scale2.value_or(at::Tensor());
     steps_ = steps;
     corr_ = corr;
-    set_slots(std::move(slots));
+    owner_ = owner;
+    put_sets(std::move(sets));
   }
-  std::vector<int32_t> slots() const { return slots_; }
-  void set_slots(std::vector<int32_t> s) {
+  std::vector<int32_t> sets() const { return sets_; }
+  void put_sets(std::vector<int32_t> s) {
     TORCH_CHECK(s.size() == numel_.size());
-    slots_ = std::move(s);
+    sets_ = std::move(s);
   }
+  bool captured() const { return captured_; }
 
   // the moments as float32 values; 32 bits: the buffers themselves
   std::pair<at::Tensor, at::Tensor> moments() const {
@@ -139,6 +141,7 @@ class Stepper {
         TORCH_CHECK(code >= 0 && p.device() == dev && given.device() == dev && given.scalar_type() == p.scalar_type() && p.numel() == numel_[i] &&
                         given.numel() == numel_[i] && p.is_contiguous(),
                     "parameter ", i, " is no longer what this optimizer was built for (device, type, size or layout changed)");
+        w.slots.push_back(i);
         if (numel_[i] == 0) continue;
         const void* g = given.const_data_ptr();
         if (!given.is_contiguous()) {
@@ -162,20 +165,23 @@ class Stepper {
     }
     if (work.empty()) return std::nullopt;
     split(active, capturing);
-    for (auto& w : work) {
-      std::vector<char> seen(numel_.size(), 0);
+    // Every tensor has a count of its own, at its own place on the device, which is advanced in every step that it takes part in.  Tensors of
+    // one set read that of the set's first, so that neighbours in memory are stepped as one run.  In a graph every block looks up its own
+    // tensor's: it is replayed when later eager steps may have parted the set.
+    std::vector<int32_t> first_of(numel_.size(), -1);
+    for (auto& w : work)
       for (auto& l : w.by_type)
         for (int32_t i : l.index) {
-          l.slot.push_back(slots_[i]);
-          if (!seen[slots_[i]]) w.slots.push_back(slots_[i]);
-          seen[slots_[i]] = 1;
+          int32_t& f = first_of[sets_[i]];
+          if (f < 0) f = i;
+          l.slot.push_back(f);
         }
-    }
+    captured_ |= capturing;
     void* stream = current_stream(dev);
     const tn_adamw_state state = {bits_, blocks_, exp_avg_.mutable_data_ptr(), exp_avg_sq_.mutable_data_ptr(),
                                   scale1_.defined() ? scale1_.mutable_data_ptr<float>() : nullptr,
                                   scale2_.defined() ? scale2_.mutable_data_ptr<float>() : nullptr, steps_.mutable_data_ptr<int32_t>(),
-                                  corr_.mutable_data_ptr<float>()};
+                                  corr_.mutable_data_ptr<float>(), capturing ? owner_.const_data_ptr<int32_t>() : nullptr};
     std::vector<std::pair<int, Lists*>> lists;
     for (auto& w : work)
       for (int code = 0; code < 3; ++code)
@@ -239,34 +245,35 @@ class Stepper {
     TORCH_CHECK_VALUE(w.h.eps >= 0.0 && w.h.weight_decay >= 0.0, "eps and weight_decay must not be negative");
   }
 
-  // Step counts belong to slots.  Where some of a slot's tensors have a gradient and others have not, those that have get a slot of
-  // their own, starting at the same count.  (There are as many slots as tensors, so one is free whenever two tensors share one.)
+  // A set holds tensors of one group whose counts are equal.  Where some of its tensors have a gradient and others have not, those that
+  // have become a set of their own.  (There are as many numbers as tensors, so one is free whenever two tensors share one.)  Sets are
+  // only ever parted once a step has been captured: a replay advances its tensors without this host code, but always all of a set.
   void split(const std::vector<char>& active, bool capturing) {
-    const size_t n = slots_.size();
+    const size_t n = sets_.size();
     std::vector<int32_t> some(n, 0), every(n, 0);
     for (size_t i = 0; i < n; ++i) {
       if (numel_[i] == 0) continue;
-      every[slots_[i]]++;
-      some[slots_[i]] += active[i];
+      every[sets_[i]]++;
+      some[sets_[i]] += active[i];
     }
     for (size_t s = 0; s < n; ++s) {
       if (some[s] == 0 || some[s] == every[s]) continue;
       TORCH_CHECK(!capturing, "AdamW: other parameters than before have gradients in a captured step: run such a step once before capturing it");
       std::vector<char> used(n, 0);
-      for (int32_t k : slots_) used[k] = 1;
+      for (int32_t k : sets_) used[k] = 1;
       size_t free = 0;
       while (used[free]) ++free;
-      steps_.narrow(0, (int64_t)free, 1).copy_(steps_.narrow(0, (int64_t)s, 1));
       for (size_t i = 0; i < n; ++i)
-        if (slots_[i] == (int32_t)s && active[i]) slots_[i] = (int32_t)free;
+        if (sets_[i] == (int32_t)s && active[i]) sets_[i] = (int32_t)free;
     }
   }
 
   int bits_;
   int64_t blocks_ = 0;
   std::vector<int64_t> numel_, first_;
-  std::vector<int32_t> slots_;
-  at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_;
+  std::vector<int32_t> sets_;
+  bool captured_ = false;
+  at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_, owner_;
 };
 
 at::Tensor grad_norm(const std::vector<at::Tensor>& tensors) {
@@ -388,7 +395,8 @@ PYBIND11_MODULE(_host, m) {
       .def("layout", &Stepper::layout)
       .def("step", &Stepper::step)
       .def("moments", &Stepper::moments)
-      .def_property("slots", &Stepper::slots, &Stepper::set_slots);
+      .def_property("sets", &Stepper::sets, &Stepper::put_sets)
+      .def_property_readonly("captured", &Stepper::captured);
   m.def("grad_norm", &grad_norm);
   m.def("quantize_rows", &quantize_rows);
   m.def("matmul_rows", &matmul_rows);

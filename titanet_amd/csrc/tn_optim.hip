@@ -82,8 +82,10 @@ __device__ double opt_power(double b, int32_t t) {       // b^t by squaring: exa
   return r;
 }
 
+constexpr int TICK_SLOTS = 512, SMALL_SLOTS = 256;     // slots that one launch can name in its arguments
+template <int MOST>
 struct OptSlots {
-  int32_t slot[256];
+  int32_t slot[MOST];
   int32_t count;
 };
 struct TickArgs {
@@ -107,14 +109,17 @@ __device__ float4 opt_tick(const TickArgs& a, int slot, bool runs) {
   return c;
 }
 
+// (the first four of the workgroup's WAVES waves add: the same order for every caller)
+template <int WAVES>
 __device__ double opt_sum_partials(const NormArgs& a) {
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < a.count; i += 256) s += a.partials[i];
-  return opt_sum_workgroup<4>(s);
+  if (threadIdx.x < 256)
+    for (int64_t i = threadIdx.x; i < a.count; i += 256) s += a.partials[i];
+  return opt_sum_workgroup<WAVES>(s);
 }
 
 __global__ __launch_bounds__(256) void grad_norm_finish_kernel(NormArgs a) {
-  const double s = opt_sum_partials(a);
+  const double s = opt_sum_partials<4>(a);
   double ctl[2];
   if (threadIdx.x == 0) {
     opt_finish_norm(a, s, ctl);
@@ -126,10 +131,10 @@ __global__ __launch_bounds__(256) void grad_norm_finish_kernel(NormArgs a) {
 }
 
 // The norm's end (first = true: from its partial sums; otherwise ctl has it) and the counts, in one launch
-__global__ __launch_bounds__(256) void adamw_tick_kernel(OptSlots list, TickArgs t, NormArgs a, bool first) {
+__global__ __launch_bounds__(TICK_SLOTS) void adamw_tick_kernel(OptSlots<TICK_SLOTS> list, TickArgs t, NormArgs a, bool first) {
   __shared__ double runs;
   if (first) {
-    const double s = opt_sum_partials(a);
+    const double s = opt_sum_partials<TICK_SLOTS / 64>(a);
     double ctl[2];
     if (threadIdx.x == 0) {
       opt_finish_norm(a, s, ctl);
@@ -167,13 +172,21 @@ __device__ __forceinline__ OptStep opt_step_of(const OptHyper& h, const float4& 
 
 // 32-bit moments: four elements to a lane, 28 bytes of an element (float parameters) moved once.  Bound by HBM: 24.7 M elements in
 // 130 us, 5.3 TB/s, where a large copy reaches 4.8; moments and gradients go past the caches (142 us with them left there).
-template <typename T>
+// EACH: a run's tensors may be at different counts, every block of 256 elements (a wave's four times 64) has the numbers of its own.
+template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, float* __restrict__ exp_avg, float* __restrict__ exp_avg_sq,
-                                                      const float* __restrict__ corr, const double* __restrict__ ctl) {
+                                                      const float* __restrict__ corr, const int32_t* __restrict__ owner,
+                                                      const double* __restrict__ ctl) {
   const int t = opt_find(list.end, OPT_LIST, blockIdx.x);
-  const float4 c = reinterpret_cast<const float4*>(corr)[list.slot[t]];
-  if (c.w == 0.f) return;
-  const OptStep step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
+  const float4* corrs = reinterpret_cast<const float4*>(corr);
+  OptStep step;
+  if constexpr (!EACH) {
+    const float4 c = corrs[list.slot[t]];
+    if (c.w == 0.f) return;
+    step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
+  } else if (ctl && ctl[1] == 0.0) {
+    return;
+  }
   const uint32_t before = t ? list.end[t - 1] : 0u;
   const int64_t lo = (int64_t)(blockIdx.x - before) * OPT_CHUNK32, n = list.numel[t];
   T* p = reinterpret_cast<T*>(list.p[t]);
@@ -186,12 +199,14 @@ __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, 
       const int64_t i = lo + k * 1024 + 4 * threadIdx.x;
       float gv[4];
       opt_load4<true, true>(g, i, n, gv);
+      if constexpr (EACH) step = opt_step_of(h, corrs[owner[list.first_block[t] + i / TN_OPT_BLOCK]], ctl ? ctl[0] : h.mult);
       opt_step32<true>(step, p, gv, i, n, m, v);
     }
   } else {
     for (int64_t i = lo + 4 * threadIdx.x; i < n; i += 1024) {
       float gv[4];
       opt_load4(g, i, n, gv);
+      if constexpr (EACH) step = opt_step_of(h, corrs[owner[list.first_block[t] + i / TN_OPT_BLOCK]], ctl ? ctl[0] : h.mult);
       opt_step32<false>(step, p, gv, i, n, m, v);
     }
   }
@@ -201,14 +216,12 @@ __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, 
 // wave and neither LDS nor a barrier is needed.  16 bytes of an element (float parameters): 64 M elements in 187 us, 5.5 TB/s.  With
 // 16-bit parameters (10 bytes) the vector pipe bounds it: some 450 instructions a block, a fifth of them in 64 bits (7.9 M bfloat16
 // elements in 26 us, 3.1 TB/s; 37 us with integer squares, 64-bit quotients and a shuffled maximum).
-template <typename T>
+template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, int8_t* __restrict__ exp_avg, uint8_t* __restrict__ exp_avg_sq,
                                                      float* __restrict__ scale1, float* __restrict__ scale2,
-                                                     const float* __restrict__ corr, const double* __restrict__ ctl) {
+                                                     const float* __restrict__ corr, const int32_t* __restrict__ owner,
+                                                     const double* __restrict__ ctl) {
   const int t = opt_find(list.end, OPT_LIST, blockIdx.x);
-  const float4 c = reinterpret_cast<const float4*>(corr)[list.slot[t]];
-  if (c.w == 0.f) return;
-  const OptStep step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
   const uint32_t before = t ? list.end[t - 1] : 0u;
   const int64_t lo = (int64_t)(blockIdx.x - before) * OPT_CHUNK8, n = list.numel[t];
   T* p = reinterpret_cast<T*>(list.p[t]);
@@ -217,6 +230,9 @@ __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, i
   const int64_t i0 = lo + (threadIdx.x >> 6) * TN_OPT_BLOCK;
   if (i0 >= n) return;
   const int64_t i = i0 + 4 * (threadIdx.x & 63), block = (int64_t)list.first_block[t] + i0 / TN_OPT_BLOCK;
+  const float4 c = reinterpret_cast<const float4*>(corr)[EACH ? (uint32_t)owner[block] : list.slot[t]];
+  if (c.w == 0.f) return;
+  const OptStep step = opt_step_of(h, c, ctl ? ctl[0] : h.mult);
   float gv[4];
   if (i0 + TN_OPT_BLOCK <= n) {
     opt_load4<true, true>(g, i, n, gv);
@@ -231,8 +247,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, i
 // with its gradient kept in registers in between.  Nothing but latency: 7.8 us for 7 bfloat16 tensors of up to 1537 elements, where the
 // three launches of the general way take 15 and the gaps between them; the call then waits for the host (11.7 us, was 22.9).
 template <typename T, int BITS>
-__global__ __launch_bounds__(1024) void adamw_small_kernel(OptList list, OptHyper h, OptSlots slots, TickArgs tick, NormArgs a, bool clip, void* exp_avg,
-                                                           void* exp_avg_sq, float* scale1, float* scale2) {
+__global__ __launch_bounds__(1024) void adamw_small_kernel(OptList list, OptHyper h, OptSlots<SMALL_SLOTS> slots, TickArgs tick, NormArgs a, bool clip, void* exp_avg,
+                                                           void* exp_avg_sq, float* scale1, float* scale2, const int32_t* owner) {
   constexpr int TURNS = SMALL_BLOCKS / 16;
   __shared__ double ctl[2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -265,9 +281,9 @@ __global__ __launch_bounds__(1024) void adamw_small_kernel(OptList list, OptHype
     const uint32_t b = k * 16 + wave;
     const int t = opt_find(list.end, OPT_LIST, b);
     if (t >= OPT_LIST || list.end[t] == 0xffffffffu) continue;
-    const float4 c = reinterpret_cast<const float4*>(tick.corr)[list.slot[t]];
-    const OptStep step = opt_step_of(h, c, ctl[0]);
     const int64_t i0 = (int64_t)(b - (t ? list.end[t - 1] : 0u)) * TN_OPT_BLOCK, first = list.first_block[t];
+    const float4 c = reinterpret_cast<const float4*>(tick.corr)[owner ? (uint32_t)owner[first + i0 / TN_OPT_BLOCK] : list.slot[t]];
+    const OptStep step = opt_step_of(h, c, ctl[0]);
     T* p = reinterpret_cast<T*>(list.p[t]);
     if constexpr (BITS == 32)
       opt_step32<false>(step, p, g[k], i0 + 4 * lane, list.numel[t], (float*)exp_avg + first * TN_OPT_BLOCK, (float*)exp_avg_sq + first * TN_OPT_BLOCK);
@@ -408,15 +424,16 @@ int lists_ok(const tn_adamw_lists* l, const tn_adamw_state* s) {
   return 0;
 }
 
-// Runs of the list, tensors that follow one another in parameters, gradients and moments joined: f(first of the run, elements).
+// Runs of the list, tensors that follow one another in parameters, gradients and moments joined (where each block knows its slot, whatever
+// the slots): f(first of the run, elements).
 template <typename F>
-int each_run(const tn_adamw_lists* l, F f) {
+int each_run(const tn_adamw_lists* l, const tn_adamw_state* s, F f) {
   const size_t size = opt_size(l->dtype);
   for (int i = 0; i < l->count;) {
     const int a = i++;
     int64_t n = l->numel[a];
     if (n == 0) continue;
-    while (i < l->count && l->numel[i] > 0 && l->slots[i] == l->slots[a] &&
+    while (i < l->count && l->numel[i] > 0 && (s->owner || l->slots[i] == l->slots[a]) &&
            l->first_block[i] * TN_OPT_BLOCK == l->first_block[a] * TN_OPT_BLOCK + n && opt_follows(l->params[a], n, size, l->params[i]) &&
            opt_follows(l->grads[a], n, size, l->grads[i]))
       n += l->numel[i++];
@@ -443,11 +460,11 @@ extern "C" int tn_adamw_tick(int32_t count, const int32_t* slots, const tn_adamw
   for (int i = 0; i < count; ++i)
     if (slots[i] < 0) return TN_E_BADARG;
   const NormArgs a = {partials, n_partials, grad_mult, max_norm, norm, ctl};
-  for (int lo = 0; lo < count || (partials && lo == 0); lo += 256) {      // (without slots the norm still ends)
-    OptSlots list;
-    list.count = std::min(256, count - lo);
+  for (int lo = 0; lo < count || (partials && lo == 0); lo += TICK_SLOTS) {      // (without slots the norm still ends)
+    OptSlots<TICK_SLOTS> list;
+    list.count = std::min(TICK_SLOTS, count - lo);
     for (int i = 0; i < list.count; ++i) list.slot[i] = slots[lo + i];
-    hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, list, tick_of(h, s->steps, s->corr), a, partials && lo == 0);
+    hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(TICK_SLOTS), 0, (hipStream_t)stream, list, tick_of(h, s->steps, s->corr), a, partials && lo == 0);
     if (const int rc = (int)hipGetLastError()) return rc;
   }
   return 0;
@@ -465,19 +482,22 @@ extern "C" int tn_adamw_apply(const tn_adamw_lists* l, const tn_adamw_state* s, 
     for (int i = used; i < OPT_LIST; ++i) list.end[i] = 0xffffffffu;
     const int rc = opt_by_type(l->dtype, [&](auto* kind) -> int {
       using T = std::remove_pointer_t<decltype(kind)>;
-      if (s->bits == 32)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw32_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult),
-                           (float*)s->exp_avg, (float*)s->exp_avg_sq, s->corr, ctl);
-      else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw8_kernel<T>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult),
-                           (int8_t*)s->exp_avg, (uint8_t*)s->exp_avg_sq, s->scale1, s->scale2, s->corr, ctl);
+      auto go = [&](auto each) {
+        if (s->bits == 32)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw32_kernel<T, decltype(each)::value>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list,
+                             hyper_of(h, grad_mult), (float*)s->exp_avg, (float*)s->exp_avg_sq, s->corr, s->owner, ctl);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(adamw8_kernel<T, decltype(each)::value>), dim3(chunks), dim3(256), 0, (hipStream_t)stream, list,
+                             hyper_of(h, grad_mult), (int8_t*)s->exp_avg, (uint8_t*)s->exp_avg_sq, s->scale1, s->scale2, s->corr, s->owner, ctl);
+      };
+      s->owner ? go(std::true_type{}) : go(std::false_type{});
       return (int)hipGetLastError();
     });
     used = 0;
     chunks = 0;
     return rc;
   };
-  const int rc = each_run(l, [&](int a, int64_t n) -> int {
+  const int rc = each_run(l, s, [&](int a, int64_t n) -> int {
     const int chunk = s->bits == 32 ? OPT_CHUNK32 : OPT_CHUNK8;
     const int64_t c = (n + chunk - 1) / chunk;
     if (c > OPT_GRID) return TN_E_UNSUPPORTED;
@@ -494,8 +514,8 @@ extern "C" int tn_adamw_step_small(const tn_adamw_lists* l, const tn_adamw_state
                                    double grad_mult, double max_norm, float* norm, void* stream) {
   if (!hyper_ok(h) || n_slots < 0 || (n_slots > 0 && !slots) || max_norm < 0.0) return TN_E_BADARG;
   if (const int rc = lists_ok(l, s)) return rc;
-  if (!s->steps || n_slots > 256) return s->steps ? TN_E_UNSUPPORTED : TN_E_BADARG;
-  OptSlots sl;
+  if (!s->steps || n_slots > SMALL_SLOTS) return s->steps ? TN_E_UNSUPPORTED : TN_E_BADARG;
+  OptSlots<SMALL_SLOTS> sl;
   sl.count = n_slots;
   for (int i = 0; i < n_slots; ++i) {
     if (slots[i] < 0) return TN_E_BADARG;
@@ -504,7 +524,7 @@ extern "C" int tn_adamw_step_small(const tn_adamw_lists* l, const tn_adamw_state
   OptList list;
   int used = 0;
   uint32_t blocks = 0;
-  const int rc = each_run(l, [&](int a, int64_t n) -> int {
+  const int rc = each_run(l, s, [&](int a, int64_t n) -> int {
     const int64_t c = (n + TN_OPT_BLOCK - 1) / TN_OPT_BLOCK;
     if (used == OPT_LIST || c > SMALL_BLOCKS || blocks + c > SMALL_BLOCKS) return TN_E_UNSUPPORTED;
     blocks += (uint32_t)c;
@@ -518,7 +538,7 @@ extern "C" int tn_adamw_step_small(const tn_adamw_lists* l, const tn_adamw_state
     using T = std::remove_pointer_t<decltype(kind)>;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, list, hyper_of(h, grad_mult), sl, tick_of(h, s->steps, s->corr), a,
-                         max_norm > 0.0, s->exp_avg, s->exp_avg_sq, s->scale1, s->scale2);
+                         max_norm > 0.0, s->exp_avg, s->exp_avg_sq, s->scale1, s->scale2, s->owner);
       return (int)hipGetLastError();
     };
     return s->bits == 32 ? go(adamw_small_kernel<T, 32>) : go(adamw_small_kernel<T, 8>);

@@ -36,7 +36,7 @@ class AdamW(torch.optim.Optimizer):
     tensors of one device.
 
     ``state_bits=32`` keeps both moments in float32, ``state_bits=8`` one byte per element and moment and a float32 scale per
-    block of 256 elements of a tensor: 2.03 bytes of state per element instead of 8.  The step itself is computed from the
+    block of 256 elements of a tensor: 2.05 bytes of state per element instead of 8.  The step itself is computed from the
     moments before they are rounded; what is rounded is what the next step starts from (forms: include/titanet_amd.h).
     Parameters of 16 bits are rounded to the nearest value after every step: updates below half a step of their type are lost.
 
@@ -61,7 +61,7 @@ class AdamW(torch.optim.Optimizer):
         self._native = _lib.load()
         self._stepper = _lib.load_host().Stepper(state_bits)      # checks, collects and launches a step
         self._list, self._device = [], None          # all parameters, group after group
-        self._exp_avg = self._exp_avg_sq = self._scale1 = self._scale2 = self._steps = self._corr = None
+        self._exp_avg = self._exp_avg_sq = self._scale1 = self._scale2 = self._steps = self._corr = self._owner = None
         self._numel = self._first = np.zeros(0, dtype=np.int64)
         self.blocks = 0
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -120,7 +120,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {g['weight_decay']}")
 
     def _extend(self, new):
-        """moments, counts and slots of the parameters of a new group, behind those there are"""
+        """moments and counts of the parameters of a new group, behind those there are"""
         if not new:
             return
         n0, b0 = len(self._list), self.blocks
@@ -129,8 +129,8 @@ class AdamW(torch.optim.Optimizer):
         first = b0 + np.concatenate([[0], np.cumsum(blocks)[:-1]]).astype(np.int64)
         self._list += new
         self._numel, self._first = np.concatenate([self._numel, numel]), np.concatenate([self._first, first])
-        # one step count for the whole group until some of its tensors go without a gradient
-        slots = self._stepper.slots + [n0] * len(new)
+        # the whole group is at one step count until some of its tensors go without a gradient
+        sets = self._stepper.sets + [n0] * len(new)
         self.blocks = b0 + int(blocks.sum())
 
         def grown(old, size, dtype):
@@ -145,8 +145,10 @@ class AdamW(torch.optim.Optimizer):
             self._scale1, self._scale2 = grown(self._scale1, self.blocks, torch.float32), grown(self._scale2, self.blocks, torch.float32)
         self._steps = grown(self._steps, len(self._list), torch.int32)
         self._corr = torch.zeros(len(self._list), 4, dtype=torch.float32, device=self._device)
-        self._stepper.layout(self._numel.tolist(), self._first.tolist(), slots, self.blocks, self._exp_avg, self._exp_avg_sq, self._scale1,
-                             self._scale2, self._steps, self._corr)
+        every = (self._numel + BLOCK - 1) // BLOCK
+        self._owner = torch.from_numpy(np.repeat(np.arange(len(every), dtype=np.int32), every)).to(self._device)      # each block's parameter
+        self._stepper.layout(self._numel.tolist(), self._first.tolist(), sets, self.blocks, self._exp_avg, self._exp_avg_sq, self._scale1,
+                             self._scale2, self._steps, self._corr, self._owner)
 
     def _groups(self):
         """(group, index of its first parameter) in order"""
@@ -200,14 +202,15 @@ class AdamW(torch.optim.Optimizer):
                   "tn_moments_encode")
 
     def _put_steps(self, steps):
-        """one slot for each group and count"""
-        slot_of, slots, counts = {}, [0] * len(self._list), torch.zeros(len(self._list), dtype=torch.int32)
+        """Sets every parameter's count.  Those of a group that are at one count are stepped together; once a step has been captured, only
+        those that were so before: replays advance what they hold, and only these are known to stay at one count."""
+        old, first, sets = self._stepper.sets, {}, [0] * len(self._list)
         for k, (group, at) in enumerate(self._groups()):
             for i in range(at, at + len(group["params"])):
-                s = slot_of.setdefault((k, steps[i]), i)
-                slots[i] = s
-                counts[s] = steps[i]
-        self._stepper.slots = slots
+                sets[i] = first.setdefault((k, steps[i], old[i] if self._stepper.captured else None), i)
+        self._stepper.sets = sets
+        counts = torch.zeros(len(self._list), dtype=torch.int32)
+        counts[:len(steps)] = torch.tensor(steps, dtype=torch.int32)
         self._steps.copy_(counts)
 
     # ------------------------------------------------------------------ checkpoints
@@ -224,12 +227,12 @@ class AdamW(torch.optim.Optimizer):
         """``torch.optim.AdamW``'s layout, the moments as they are held: float32, or int8 / uint8 codes with ``exp_avg_scale`` /
         ``exp_avg_sq_scale`` per block of 256 elements.  Parameters that were never stepped have no entry."""
         state, groups = {}, []
-        counts, slots = (self._steps.cpu().tolist(), self._stepper.slots) if self._device is not None else ([], [])
+        counts = self._steps.cpu().tolist() if self._device is not None else []
         for group, at in self._groups():
             index = list(range(at, at + len(group["params"])))
             groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": index})
             for i in index:
-                t = counts[slots[i]]
+                t = counts[i]
                 if t:
                     state[i] = {"step": torch.tensor(float(t)), **self._views(i)}
         return {"state": state, "param_groups": groups}
