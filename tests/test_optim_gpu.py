@@ -592,3 +592,37 @@ def test_a_graph_and_steps_of_some_tensors_count_together(bits):
     some(1)
     replay(first)
     some(0, 1, 2, 3)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_group_is_added_once_a_step_is_captured(bits):
+    """a graph writes the buffers that the optimizer had when it was captured: these stay where they are"""
+    p, q = _tensors([300], torch.float32, 41)[0], _tensors([300], torch.float32, 41)[0]
+    opt, eager = (AdamW([x], lr=torch.full((), 1e-2, device="cuda"), state_bits=bits) for x in (p, q))
+    p.grad = q.grad = _grads([300], torch.float32, 42)[0]
+    opt.step()
+    eager.step()
+    late = _tensors([70], torch.float32, 43)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    held = [x.data_ptr() for x in (opt._exp_avg, opt._exp_avg_sq, opt._steps, opt._corr, opt._owner)]
+    with pytest.raises(RuntimeError, match="add all groups before"):
+        opt.add_param_group({"params": [late]})
+    assert held == [x.data_ptr() for x in (opt._exp_avg, opt._exp_avg_sq, opt._steps, opt._corr, opt._owner)] and len(opt.param_groups) == 1
+    opt.load_state_dict(opt.state_dict())
+    assert held == [x.data_ptr() for x in (opt._exp_avg, opt._exp_avg_sq, opt._steps, opt._corr, opt._owner)]
+    for _ in range(3):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(opt.moments(), eager.moments()))
+    wide = []
+    for x, o in ((p, opt), (q, eager)):                                                   # the way there is
+        wide.append(AdamW([{"params": [x]}, {"params": [late.clone()]}], lr=1e-2, state_bits=bits))
+        state = o.state_dict()
+        wide[-1].load_state_dict({"state": state["state"], "param_groups": [state["param_groups"][0], {"params": [1]}]})
+        wide[-1].param_groups[1]["params"][0].grad = torch.ones_like(late)
+        wide[-1].step()
+        assert {i: int(e["step"]) for i, e in wide[-1].state_dict()["state"].items()} == {0: 5, 1: 1}
+    assert torch.equal(p, q)

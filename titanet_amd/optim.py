@@ -49,7 +49,10 @@ class AdamW(torch.optim.Optimizer):
     ``grad_mult`` multiplies the gradients before everything else (1 / world size behind a summing all-reduce).
 
     ``lr`` may be a 0-dim float32 tensor on the device; a step can be captured into a graph only then (a number would be frozen
-    into the graph).  Parameters whose ``.grad`` is None are left alone and keep a step count of their own."""
+    into the graph).  The graph then reads and writes the optimizer's buffers: keep the optimizer as long as the graph.  No
+    parameter group can be added any more; loading a state and eager steps of all or some parameters go on as before.
+
+    Parameters whose ``.grad`` is None are left alone and keep a step count of their own."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, grad_mult=1.0):
         if state_bits not in (8, 32):
@@ -71,6 +74,9 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ layout
     def add_param_group(self, param_group):
+        if self._stepper.captured:
+            raise RuntimeError("AdamW: a captured step holds this optimizer's moments, which a new group would move: add all groups before "
+                               "capturing a step, or load state_dict() into a new optimizer")
         params = param_group["params"]
         params = [params] if isinstance(params, torch.Tensor) else list(params)
         new = [p[1] if isinstance(p, tuple) else p for p in params]
