@@ -6,7 +6,7 @@ import torch
 
 from titanet_amd import LOSSES, TitaNet, metrics
 from titanet_amd.int8 import quantize_rows
-from titanet_amd.optim import AdamW
+from titanet_amd.optim import AdamW, grad_norm
 from titanet_amd.train import load_checkpoint, save_checkpoint
 from titanet_amd.trainer import Trainer
 
@@ -120,3 +120,13 @@ def test_train_with_8_bit_moments_then_answer_in_8_bits(loss):
     (m32, s32, labels), (m8, s8, _) = (metrics.verification_test(model, specs, ids, score_bits=b) for b in (32, 8))
     assert s32.shape == s8.shape == (1600,) and np.abs(s32 - s8).max() < 0.02 and set(m8) == set(m32)
     assert model.training is False
+
+
+def test_trainer_graphs_of_several_lengths_report_their_own_norm():
+    model = _model()
+    trainer = Trainer(model, lr=1e-3, optimizer="adamw", max_grad_norm=1.0, use_graph=True, graph_warmup=1)
+    for k, frames in enumerate((64, 96, 64, 96, 64, 64, 96, 96, 64)):
+        trainer.step(*_batch(frames=frames, seed=20 + k))
+        want = float(grad_norm(model.flat_gradients()))
+        assert abs(float(trainer.last_grad_norm) - want) <= 2 * 2.0 ** -24 * want, (k, frames)
+    assert all(st["graph"] is not None for st in trainer._graphs.values())

@@ -626,3 +626,35 @@ def test_no_group_is_added_once_a_step_is_captured(bits):
         wide[-1].step()
         assert {i: int(e["step"]) for i, e in wide[-1].state_dict()["state"].items()} == {0: 5, 1: 1}
     assert torch.equal(p, q)
+
+
+def test_the_last_norm_is_the_last_steps_whoever_ran_it():
+    p, q = _tensors([5000], torch.float32, 25)[0], _tensors([5000], torch.float32, 25)[0]
+    opt, eager = (AdamW([x], lr=torch.full((), 1e-2, device="cuda"), max_grad_norm=1.0) for x in (p, q))
+    grads, graphs = [2.0 ** k * x for k, x in enumerate(_grads([5000] * 3, torch.float32, 26))], []
+    norms = []
+    for g in grads:                                              # norms of eager steps can be collected
+        p.grad = q.grad = g
+        opt.step()
+        eager.step()
+        norms.append(opt.last_grad_norm)
+    assert len({float(n) for n in norms}) == 3
+    for g in grads:
+        p.grad = g
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            opt.step()
+    for k in (0, 1, 2, 3, 1, 0, 3, 2):
+        if k < 3:
+            graphs[k].replay()
+            q.grad = grads[k]
+        else:
+            p.grad = q.grad = grads[0] * 0.5
+            opt.step()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q) and torch.equal(opt.last_grad_norm, eager.last_grad_norm), k
+    grads[1][3] = float("nan")                                  # a skipped replay says so
+    graphs[0].replay()
+    graphs[1].replay()
+    assert not float(opt.last_grad_norm) < float("inf")

@@ -89,6 +89,7 @@ class Stepper {
     steps_ = steps;
     corr_ = corr;
     owner_ = owner;
+    if (!norm_.defined()) norm_ = at::zeros({}, corr.options());
     put_sets(std::move(sets));
   }
   std::vector<int32_t> sets() const { return sets_; }
@@ -187,7 +188,9 @@ class Stepper {
       for (int code = 0; code < 3; ++code)
         if (!w.by_type[code].p.empty()) lists.emplace_back(code, &w.by_type[code]);
     at::Tensor norm, partials;
-    if (max_norm > 0.0) norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    // A tensor of its own for every eager step, so that norms can be collected; once there is a graph, one that every step and replay writes:
+    // the host does not see which of several graphs ran last.
+    if (max_norm > 0.0) norm = captured_ ? norm_ : at::empty({}, norm_.options());
     float* norm_ptr = norm.defined() ? norm.mutable_data_ptr<float>() : nullptr;
     int small = TN_E_UNSUPPORTED;
     if (lists.size() == 1) {
@@ -273,7 +276,7 @@ class Stepper {
   std::vector<int64_t> numel_, first_;
   std::vector<int32_t> sets_;
   bool captured_ = false;
-  at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_, owner_;
+  at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_, owner_, norm_;
 };
 
 at::Tensor grad_norm(const std::vector<at::Tensor>& tensors) {

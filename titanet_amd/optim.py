@@ -42,7 +42,7 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_grad_norm``: the gradients of all groups together are scaled to at most this 2-norm, as
     ``torch.nn.utils.clip_grad_norm_`` does (the ``.grad`` tensors themselves keep their values); ``last_grad_norm`` is the norm
-    before that, on the device.  A norm that is not finite skips the step — parameters, moments and step counts stay as they
+    before that, on the device (once a step has been captured: one tensor that every step and replay writes).  A norm that is not finite skips the step — parameters, moments and step counts stay as they
     are; without ``max_grad_norm`` a gradient that is NaN or infinite reaches its element (8 bits: its block of 256).
     ``float("inf")`` measures the norm and skips, without scaling.
 

@@ -188,7 +188,8 @@ class Trainer:
 
     @property
     def last_grad_norm(self):
-        """the gradient's norm before clipping (0-dim device tensor; AdamW with ``max_grad_norm``, else None)"""
+        """the last step's gradient norm before clipping (0-dim device tensor, with ``use_graph`` one that every step writes; AdamW with
+        ``max_grad_norm``, else None)"""
         return self.adamw.last_grad_norm if self.adamw is not None else None
 
     def optimizer_step(self):
