@@ -260,7 +260,8 @@ int tn_moments_encode(const float* in1, const float* in2, void* exp_avg, void* e
 /* ---- matrix product in 8-bit integers with a scale for each token and each channel (new; the reference multiplies in float32,
  * nn.Linear of src/losses.py:30 and the cosine scores of src/learn.py:441-447) --------------------------------------------------
  *   y[m][n] = a_scales[m] b_scales[n] sum_k a[m][k] b[n][k] (+ bias[n])           the sum in 32-bit integers, exact
- * Codes are int8 [rows][ld], ld a multiple of 64, base 16-byte aligned, zeros from k to the next multiple of 64.
+ * Codes are int8 [rows][ld], ld a multiple of 64, base 16-byte aligned, zeros from k to the next multiple of 64.  Products of more than
+ * a few rows take ld up to (2^31 - 1) / 128 and return TN_E_UNSUPPORTED beyond, with nothing launched.
  * tn_int8_quantize_rows makes them from float rows of any stride: scale = max(max |row| / 127, 2^-126) (0 for a row of zeros), code
  * = x / scale rounded to the nearest integer, even half way; a row with a NaN or an infinity gets the scale NaN and codes 0 (its
  * products are NaN). */

@@ -60,3 +60,17 @@ def test_c_entries_refuse_before_they_touch_the_device():
     need = lib.tn_int8_linear_workspace(100, 3)
     assert need == 100 * 64 + 400 and lib.tn_int8_linear_workspace(4, 3) == 0 and lib.tn_int8_linear_workspace(4, 0) == bad
     assert linear(m=100) == bad and linear(m=100, ws=at, size=need - 1) == bad and linear(m=100, ws=C.c_void_p(4104), size=need) == bad
+
+
+def test_tiles_refuse_rows_further_apart_than_they_can_address():
+    """128 rows of a tile have to lie within 2^31 - 1 bytes: a pitch beyond that is refused before anything is launched"""
+    lib = _lib.load()
+    at, none, unsupported = C.c_void_p(4096), C.c_void_p(0), -2
+    most = (2 ** 31 - 1) // 128 // 64 * 64
+    for lda, ldb in ((most + 64, 64), (64, most + 64), (2 ** 25, 64), (64, 2 ** 33), (2 ** 40, 2 ** 40)):
+        for m, k in ((33, 3), (100, 64), (4, 20000)):
+            lda_, ldb_ = max(lda, 20032), max(ldb, 20032)
+            assert lib.tn_int8_matmul(at, at, lda_, at, at, ldb_, none, at, 0, 5, m, 5, k, none) == unsupported
+            if ldb_ > most:
+                size = lib.tn_int8_linear_workspace(m, k)
+                assert lib.tn_int8_linear(at, 0, k, at, at, ldb_, none, at, 0, 5, m, 5, k, at, size, none) == unsupported

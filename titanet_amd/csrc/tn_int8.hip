@@ -468,6 +468,8 @@ int q8_by_type(int dtype, F f) {
 constexpr int64_t Q8_GRID = (1 << 24) - 1;
 constexpr int64_t Q8_FEW = 32;                     // rows of the kernel that makes their codes itself
 constexpr int64_t Q8_FEW_LDS = 64 * 1024;          // ... where these fit
+constexpr int Q8_TILE = 128;                       // rows and columns of a tile
+constexpr int64_t Q8_PITCH = 0x7fffffff / Q8_TILE; // most bytes from row to row of its operands: a descriptor spans 2^31 - 1 bytes, offsets are 32 bits
 
 int64_t q8_padded(int64_t k) { return (k + 63) / 64 * 64; }
 bool q8_few(int64_t m, int64_t k) { return m <= Q8_FEW && m * (q8_padded(k) + 16) <= Q8_FEW_LDS; }
@@ -501,8 +503,9 @@ int q8_few_rows(const FewArgs& f, void* stream) {
 
 template <typename Y>
 int q8_tiles(const Int8Args& g, void* stream) {
+  if (g.lda > Q8_PITCH || g.ldb > Q8_PITCH) return TN_E_UNSUPPORTED;
   auto go = [&](auto step, bool down) -> int {
-    constexpr int T = 128, STEP = decltype(step)::value, NS = 2;
+    constexpr int T = Q8_TILE, STEP = decltype(step)::value, NS = 2;
     const int64_t a = (g.m + T - 1) / T, b = (g.n + T - 1) / T;
     if (b > Q8_GRID || a > Q8_GRID / b) return TN_E_UNSUPPORTED;
     return q8_launch(int8_tile_kernel<Y, T, T, STEP, NS>, dim3((unsigned)(a * b)), 256, (size_t)NS * 2 * T * STEP, stream, g, (int)a, (int)b, down);
@@ -512,7 +515,7 @@ int q8_tiles(const Int8Args& g, void* stream) {
   // 192 173 / 214 and 76800 x 1536 x 1536 291 / 314 (bf16 outputs).  Short sums of few rows are bound by their stores: steps of 64 bytes
   // leave room for twice the workgroups (250 x 100003 x 192 21.3 us, 1000 x 50000 x 192 30.1); everything else takes whole lines of
   // 128 (4708 x 50021 x 192 173 against 199 us, 76800 x 1536 x 1536 291 against 328, 2048 x 2048 x 2048 17 against 19).
-  const bool down = g.m <= 8 * 128;
+  const bool down = g.m <= 8 * Q8_TILE;
   return down && g.k <= 512 ? go(std::integral_constant<int, 64>{}, down) : go(std::integral_constant<int, 128>{}, down);
 }
 
@@ -581,6 +584,7 @@ extern "C" int tn_int8_linear(const void* x, int32_t x_dtype, int64_t ldx, const
       return q8_by_type(y_dtype, [&](auto* ky) -> int { return q8_few_rows<X, std::remove_pointer_t<decltype(ky)>>(FewArgs{x, g, ldx, (int)k}, stream); });
     });
   }
+  if (ldb > Q8_PITCH) return TN_E_UNSUPPORTED;
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < tn_int8_linear_workspace(m, k)) return TN_E_BADARG;
   const int64_t ld = q8_padded(k);
   float* scales = reinterpret_cast<float*>((char*)workspace + m * ld);
