@@ -74,3 +74,17 @@ def test_tiles_refuse_rows_further_apart_than_they_can_address():
             if ldb_ > most:
                 size = lib.tn_int8_linear_workspace(m, k)
                 assert lib.tn_int8_linear(at, 0, k, at, at, ldb_, none, at, 0, 5, m, 5, k, at, size, none) == unsupported
+
+
+def test_products_of_operands_that_left_the_device():
+    """rows and layers whose buffers were moved to the host: refused before a kernel gets their addresses"""
+    rows = Int8Rows._of(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4), 3)
+    layer = Int8Linear.__new__(Int8Linear)
+    torch.nn.Module.__init__(layer)
+    layer.in_features, layer.out_features = 3, 4
+    for name, t in (("codes", rows._padded), ("scales", rows.scales), ("bias", torch.zeros(4))):
+        layer.register_buffer(name, t)
+    for call in (lambda: int8_matmul(torch.ones(2, 3), rows), lambda: int8_matmul(torch.ones(64, 3), rows), lambda: int8_matmul(rows, rows),
+                 lambda: layer(torch.ones(2, 3)), lambda: layer(torch.ones(64, 3, dtype=torch.bfloat16)), lambda: layer(torch.ones(0, 3))):
+        with pytest.raises(RuntimeError, match="no CPU execution path"):
+            call()

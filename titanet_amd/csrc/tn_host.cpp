@@ -325,6 +325,19 @@ std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& given) {
   return {codes, scales};
 }
 
+// Rows of codes as the kernels read them.  A module's buffers can be moved or replaced after they were checked: a kernel that gets a host
+// address takes the device down.
+void need_rows(const at::Tensor& codes, const at::Tensor& scales, int64_t cols, const char* what) {
+  TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), "titanet_amd.int8: ", what, " must be on a ROCm device, got ", codes.device(), " and ", scales.device(),
+              "; there is no CPU execution path");
+  TORCH_CHECK_VALUE(codes.device() == scales.device(), "codes and scales are on different devices: ", codes.device(), " and ", scales.device());
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kChar && scales.scalar_type() == at::kFloat, what, " must be int8 codes and float32 scales, got ", codes.scalar_type(),
+                   " and ", scales.scalar_type());
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.is_contiguous() && codes.size(1) >= cols && scales.dim() == 1 && scales.is_contiguous() &&
+                        scales.size(0) == codes.size(0),
+                    what, ": codes ", codes.sizes(), " and scales ", scales.sizes(), " do not belong together");
+}
+
 struct Out {
   at::Tensor bias, y;
   const float* bias_ptr = nullptr;
@@ -355,6 +368,8 @@ void product(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& 
 
 at::Tensor matmul_rows(const at::Tensor& a, const at::Tensor& a_scales, int64_t cols_a, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols,
                        const std::optional<at::Tensor>& bias, std::optional<c10::ScalarType> out) {
+  need_rows(a, a_scales, cols_a, "the first operand");
+  need_rows(b, b_scales, cols, "the second operand");
   const c10::OptionalDeviceGuard guard(b.device());
   TORCH_CHECK(!(at::GradMode::is_enabled() && bias && bias->requires_grad()), "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
   const at::NoGradGuard no_grad;
@@ -368,6 +383,7 @@ at::Tensor matmul_float(const at::Tensor& x, const at::Tensor& b, const at::Tens
   TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0 && x.layout() == at::kStrided,
                    "the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1, "the first operand needs at least one dimension");
+  need_rows(b, b_scales, cols, "the second operand");
   TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias && bias->requires_grad()))),
               "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
   const at::NoGradGuard no_grad;
