@@ -263,3 +263,21 @@ def test_products_at_the_ends_of_the_few_rows_kernel(m, k):
         want, part = O.product(*O.quantize(_np(x)), *O.quantize(_np(w)))
         for a in (x, quantize_rows(x)):
             _compare(int8_matmul(a, quantize_rows(w)), want, part, "fp32")
+
+
+def test_gradients_are_not_dropped():
+    x, w = _x(3, 8, 2).requires_grad_(True), quantize_rows(_x(4, 8, 1))
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        quantize_rows(x)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        quantize_rows(x * 2)
+    scales = torch.ones(4, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        Int8Rows(w.codes, scales)
+    with torch.no_grad():
+        assert int8_matmul(quantize_rows(x), Int8Rows(w.codes, scales)).shape == (3, 4)
+    assert quantize_rows(x.detach()).shape == (3, 8)
+    layer = Int8Linear(torch.nn.Parameter(_x(4, 8, 1)), torch.nn.Parameter(torch.ones(4, device="cuda")))     # weights are laid out once, for serving
+    assert layer(x.detach()).shape == (3, 4)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        layer(x)

@@ -309,12 +309,18 @@ at::Tensor grad_norm(const std::vector<at::Tensor>& tensors) {
 }
 
 // --------------------------------------------------------------------------------------------------------- 8-bit product
+// what flows through these operators is not differentiated: an operand that asks for it is refused, not cut off
+void need_no_gradient(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no backward pass: detach its operands or call it under torch.no_grad()");
+}
+
 std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& given) {
-  const at::NoGradGuard no_grad;
   TORCH_CHECK_TYPE(type_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "quantize_rows takes a float32, bfloat16 or float16 matrix, got ", given.scalar_type());
   TORCH_CHECK_VALUE(given.dim() == 2 && given.size(1) >= 1, "quantize_rows takes a matrix with at least one column, got ", given.sizes());
   TORCH_CHECK_VALUE(given.size(1) <= TN_INT8_MAX_K, "rows of more than ", TN_INT8_MAX_K, " values could overflow the 32-bit sums");
   TORCH_CHECK(given.is_cuda(), "titanet_amd.int8: x must be a ROCm device tensor; there is no CPU execution path");
+  need_no_gradient(given, "quantize_rows");
+  const at::NoGradGuard no_grad;
   const c10::OptionalDeviceGuard guard(given.device());
   const at::Tensor x = given.stride(1) == 1 || given.size(1) == 1 ? given : given.contiguous();
   const int64_t rows = x.size(0), cols = x.size(1), ld = (cols + 63) / 64 * 64;
@@ -371,7 +377,7 @@ at::Tensor matmul_rows(const at::Tensor& a, const at::Tensor& a_scales, int64_t 
   need_rows(a, a_scales, cols_a, "the first operand");
   need_rows(b, b_scales, cols, "the second operand");
   const c10::OptionalDeviceGuard guard(b.device());
-  TORCH_CHECK(!(at::GradMode::is_enabled() && bias && bias->requires_grad()), "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
+  if (bias) need_no_gradient(*bias, "int8_matmul");
   const at::NoGradGuard no_grad;
   Out o = prepare_out(a.device(), cols_a, cols, a.size(0), b, bias, out.value_or(at::kFloat));
   product(a, a_scales, b, b_scales, cols, o);
@@ -384,8 +390,8 @@ at::Tensor matmul_float(const at::Tensor& x, const at::Tensor& b, const at::Tens
                    "the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1, "the first operand needs at least one dimension");
   need_rows(b, b_scales, cols, "the second operand");
-  TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias && bias->requires_grad()))),
-              "int8_matmul has no backward pass: detach its operands or call it under torch.no_grad()");
+  need_no_gradient(x, "int8_matmul");
+  if (bias) need_no_gradient(*bias, "int8_matmul");
   const at::NoGradGuard no_grad;
   const c10::OptionalDeviceGuard guard(b.device());
   const int64_t cols_a = x.size(-1);

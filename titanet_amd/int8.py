@@ -36,6 +36,8 @@ class Int8Rows:
         _need_device(codes, "codes")
         if scales.device != codes.device:
             raise ValueError(f"codes and scales are on different devices: {codes.device} and {scales.device}")
+        if torch.is_grad_enabled() and scales.requires_grad:
+            raise RuntimeError("Int8Rows has no backward pass: detach its scales or build it under torch.no_grad()")
         rows, cols = codes.shape
         padded = torch.zeros(rows, (cols + 63) // 64 * 64, dtype=torch.int8, device=codes.device)
         padded[:, :cols] = codes.detach()
@@ -69,7 +71,8 @@ class Int8Rows:
 
 def quantize_rows(x):
     """``Int8Rows`` of a float matrix (float32, bfloat16 or float16): scale max |row| / 127 (at least 2^-126; 0 for a row of
-    zeros), codes the nearest integers to x / scale, even half way.  A row with a NaN or an infinity gets the scale NaN."""
+    zeros), codes the nearest integers to x / scale, even half way.  A row with a NaN or an infinity gets the scale NaN.  There is no backward
+    pass: a matrix that needs a gradient is refused outside ``torch.no_grad()``."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"quantize_rows takes a float32, bfloat16 or float16 matrix, got {type(x).__name__}")
     padded, scales = _lib.load_host().quantize_rows(x)
@@ -94,7 +97,7 @@ class Int8Linear(nn.Module):
 
     def __init__(self, weight, bias=None):
         super().__init__()
-        rows = quantize_rows(weight)
+        rows = quantize_rows(weight.detach())
         self.in_features, self.out_features = rows.cols, len(rows)
         self.register_buffer("codes", rows._padded)
         self.register_buffer("scales", rows.scales)

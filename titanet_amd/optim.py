@@ -27,7 +27,8 @@ def _dev(tensor):
 
 def grad_norm(tensors):
     """The 2-norm of all elements of ``tensors`` together, as a 0-dim float32 tensor on their device.  Summed in 64 bits in a
-    fixed order: two calls on the same values give the same number.  float32, bfloat16 and float16 may be mixed."""
+    fixed order: two calls on the same values give the same number.  float32, bfloat16 and float16 may be mixed.  The number is for
+    reading: it takes no part in autograd."""
     return _lib.load_host().grad_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors))
 
 
