@@ -6,6 +6,7 @@ half a step of a 16-bit output."""
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from tests import int8_oracle as O
 from titanet_amd import LOSSES
@@ -281,3 +282,18 @@ def test_gradients_are_not_dropped():
     assert layer(x.detach()).shape == (3, 4)
     with pytest.raises(RuntimeError, match="no backward pass"):
         layer(x)
+
+
+def test_tangents_are_not_dropped():
+    x, w, bias = _x(3, 8, 2), quantize_rows(_x(4, 8, 1)), torch.ones(4, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            int8_matmul(dual, w)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            quantize_rows(dual)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            int8_matmul(x, w, bias=forward_ad.make_dual(bias, bias))
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            int8_matmul(quantize_rows(x), w, bias=forward_ad.make_dual(bias, bias))
+        assert int8_matmul(x, w, bias=bias).shape == (3, 4)

@@ -312,6 +312,7 @@ at::Tensor grad_norm(const std::vector<at::Tensor>& tensors) {
 // what flows through these operators is not differentiated: an operand that asks for it is refused, not cut off
 void need_no_gradient(const at::Tensor& t, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no backward pass: detach its operands or call it under torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, " has no backward pass and no forward-mode derivative: unpack its operands' primals");
 }
 
 std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& given) {
