@@ -297,3 +297,12 @@ def test_tangents_are_not_dropped():
         with pytest.raises(RuntimeError, match="no backward pass"):
             int8_matmul(quantize_rows(x), w, bias=forward_ad.make_dual(bias, bias))
         assert int8_matmul(x, w, bias=bias).shape == (3, 4)
+
+
+def test_a_product_is_not_traced():
+    x = _x(3, 8, 2)
+    layer = Int8Linear(_x(4, 8, 1))
+    for call in (layer, lambda a: int8_matmul(quantize_rows(a), quantize_rows(x)), lambda a: quantize_rows(a).codes):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x, check_trace=False)
+    assert layer(x).shape == (3, 4)

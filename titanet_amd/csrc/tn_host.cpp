@@ -10,6 +10,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -315,7 +316,13 @@ void need_no_gradient(const at::Tensor& t, const char* what) {
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, " has no backward pass and no forward-mode derivative: unpack its operands' primals");
 }
 
+// torch.jit.trace records torch's own operators only: a module traced through here would return memory that nothing has written
+void need_no_trace(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced (torch.jit.trace, torch.onnx.export): its kernels are no operators of torch");
+}
+
 std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& given) {
+  need_no_trace("quantize_rows");
   TORCH_CHECK_TYPE(type_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "quantize_rows takes a float32, bfloat16 or float16 matrix, got ", given.scalar_type());
   TORCH_CHECK_VALUE(given.dim() == 2 && given.size(1) >= 1, "quantize_rows takes a matrix with at least one column, got ", given.sizes());
   TORCH_CHECK_VALUE(given.size(1) <= TN_INT8_MAX_K, "rows of more than ", TN_INT8_MAX_K, " values could overflow the 32-bit sums");
@@ -375,6 +382,7 @@ void product(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& 
 
 at::Tensor matmul_rows(const at::Tensor& a, const at::Tensor& a_scales, int64_t cols_a, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols,
                        const std::optional<at::Tensor>& bias, std::optional<c10::ScalarType> out) {
+  need_no_trace("int8_matmul");
   need_rows(a, a_scales, cols_a, "the first operand");
   need_rows(b, b_scales, cols, "the second operand");
   const c10::OptionalDeviceGuard guard(b.device());
@@ -387,6 +395,7 @@ at::Tensor matmul_rows(const at::Tensor& a, const at::Tensor& a_scales, int64_t 
 
 at::Tensor matmul_float(const at::Tensor& x, const at::Tensor& b, const at::Tensor& b_scales, int64_t cols, const std::optional<at::Tensor>& bias,
                         std::optional<c10::ScalarType> out) {
+  need_no_trace("int8_matmul");
   TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0 && x.layout() == at::kStrided,
                    "the first operand must be Int8Rows or a float32, bfloat16 or float16 tensor, got ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1, "the first operand needs at least one dimension");
