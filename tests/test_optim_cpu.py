@@ -101,3 +101,21 @@ def test_oracle_codes_are_the_nearest_and_survive_a_round_trip():
         step = 1 / 255 if second else 1 / 127
         assert off[code != 1].max() <= step / 2 * (1 + 1e-6) and off.max() <= step
         assert not second or (code[y > 0] >= 1).all()
+
+
+def test_hooks_of_a_state_dict_run_in_torchs_order():
+    """the same calls on torch's own optimizer and on this one, where there is no parameter that would need a device"""
+    seen = []
+    for opt in (torch.optim.AdamW([{"params": []}]), AdamW([{"params": []}])):
+        calls = []
+        seen.append(calls)
+        opt.register_state_dict_pre_hook(lambda o: calls.append("pre"))
+        opt.register_state_dict_post_hook(lambda o, sd: calls.append(("post", sorted(sd))))
+        opt.register_state_dict_post_hook(lambda o, sd: {**sd, "epoch": 4}, prepend=True)
+        opt.register_load_state_dict_pre_hook(lambda o, sd: calls.append(("before", sorted(sd))))
+        opt.register_load_state_dict_pre_hook(lambda o, sd: {k: v for k, v in sd.items() if k != "epoch"}, prepend=True)
+        opt.register_load_state_dict_post_hook(lambda o: calls.append("loaded"))
+        sd = opt.state_dict()
+        opt.load_state_dict(sd)
+        assert sd["epoch"] == 4
+    assert seen[0] == seen[1] and len(seen[0]) == 4

@@ -658,3 +658,26 @@ def test_the_last_norm_is_the_last_steps_whoever_ran_it():
     graphs[0].replay()
     graphs[1].replay()
     assert not float(opt.last_grad_norm) < float("inf")
+
+
+def test_state_dict_hooks_are_called():
+    p = torch.ones(300, device="cuda")
+    opt, calls = AdamW([p]), []
+    p.grad = torch.ones(300, device="cuda")
+    opt.step()
+    opt.register_state_dict_pre_hook(lambda o: calls.append("pre"))
+    opt.register_state_dict_post_hook(lambda o, sd: calls.append("post"))
+    handle = opt.register_state_dict_post_hook(lambda o, sd: {**sd, "epoch": 4})
+    sd = opt.state_dict()
+    assert calls == ["pre", "post"] and sd["epoch"] == 4 and set(sd["state"]) == {0}
+    handle.remove()
+    assert "epoch" not in opt.state_dict()
+
+    def twice(o, given):
+        calls.append("before loading")
+        return {"state": {0: {**given["state"][0], "step": torch.tensor(9.0)}}, "param_groups": given["param_groups"]}
+    opt.register_load_state_dict_pre_hook(twice)
+    opt.register_load_state_dict_post_hook(lambda o: calls.append("loaded"))
+    opt.load_state_dict(sd)
+    assert calls[-2:] == ["before loading", "loaded"] and int(sd["state"][0]["step"]) == 1
+    assert int(opt.state_dict()["state"][0]["step"]) == 9

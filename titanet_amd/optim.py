@@ -232,7 +232,10 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self):
         """``torch.optim.AdamW``'s layout, the moments as they are held: float32, or int8 / uint8 codes with ``exp_avg_scale`` /
-        ``exp_avg_sq_scale`` per block of 256 elements.  Parameters that were never stepped have no entry."""
+        ``exp_avg_sq_scale`` per block of 256 elements.  Parameters that were never stepped have no entry.  (``self.state`` stays empty:
+        the moments of all parameters lie in buffers of the whole list.)  Hooks registered on the optimizer are called as torch does."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         state, groups = {}, []
         counts = self._steps.cpu().tolist() if self._device is not None else []
         for group, at in self._groups():
@@ -242,12 +245,25 @@ class AdamW(torch.optim.Optimizer):
                 t = counts[i]
                 if t:
                     state[i] = {"step": torch.tensor(float(t)), **self._views(i)}
-        return {"state": state, "param_groups": groups}
+        state_dict = {"state": state, "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            given = hook(self, state_dict)
+            state_dict = state_dict if given is None else given
+        return state_dict
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes the dict of :meth:`state_dict` of either width, or of ``torch.optim.AdamW`` / ``torch.optim.Adam``: moments held in
-        another width are converted."""
+        another width are converted.  Hooks registered on the optimizer are called as torch does."""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            given = hook(self, state_dict)
+            state_dict = state_dict if given is None else given
+        self._load_state_dict(state_dict)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
+
+    @torch.no_grad()
+    def _load_state_dict(self, state_dict):
         groups, state = state_dict["param_groups"], state_dict["state"]
         if len(groups) != len(self.param_groups) or any(len(g["params"]) != len(o["params"]) for g, o in zip(groups, self.param_groups)):
             raise ValueError("loaded state dict has other parameter groups than this optimizer")
