@@ -681,3 +681,20 @@ def test_state_dict_hooks_are_called():
     opt.load_state_dict(sd)
     assert calls[-2:] == ["before loading", "loaded"] and int(sd["state"][0]["step"]) == 1
     assert int(opt.state_dict()["state"][0]["step"]) == 9
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_lies_between_loaded_moments_is_left_out(bits):
+    sizes = [300, 7, 256]
+    params = _tensors(sizes, torch.float32, 38)
+    opts = [AdamW(params, state_bits=bits) for _ in range(2)]
+    live = torch.zeros(opts[0].blocks * BLOCK, dtype=torch.bool, device="cuda")
+    for first, n in zip(opts[0]._first, sizes):
+        live[first * BLOCK:first * BLOCK + n] = True
+    for fill in (float("nan"), float("inf"), -3.0):
+        for opt, between in zip(opts, (0.0, fill)):
+            m, v = (torch.full((len(live),), between, device="cuda") for _ in range(2))
+            m[live], v[live] = _tensors([563], torch.float32, 39)[0], _tensors([563], torch.float32, 40)[0].abs()
+            opt.load_moments(m, v, step=1)
+        for a, b in zip(opts[0].moments(), opts[1].moments()):
+            assert torch.equal(a, b) and not b[~live].any()

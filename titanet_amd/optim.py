@@ -178,23 +178,25 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ moments as values
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters as flat float32 tensors: parameter i's from ``BLOCK * first`` on, every
-        parameter at a multiple of 256, zeros between them.  32 bits: the buffers themselves; 8 bits: the values of the codes."""
+        parameter at a multiple of 256, zeros between them (8 bits: NaN in the rest of a block that is NaN).  32 bits: the buffers
+        themselves; 8 bits: the values of the codes."""
         return self._stepper.moments() if self._device is not None else (self._exp_avg, self._exp_avg_sq)
 
     @torch.no_grad()
     def load_moments(self, exp_avg, exp_avg_sq, step):
-        """Sets the moments from two flat tensors laid out as :meth:`moments` gives them, and every step count to ``step``."""
+        """Sets the moments from two flat tensors laid out as :meth:`moments` gives them, and every step count to ``step``.  What lies
+        between the parameters is not read."""
         size = self.blocks * BLOCK
         if tuple(exp_avg.shape) != (size,) or tuple(exp_avg_sq.shape) != (size,):
             raise ValueError(f"moments of this optimizer are two tensors of {size} values, got {tuple(exp_avg.shape)} and {tuple(exp_avg_sq.shape)}")
         if not 0 <= int(step) < 2 ** 31:
             raise ValueError(f"step must be a count, got {step}")
         m, v = (t.detach().to(device=self._device, dtype=torch.float32, copy=True) for t in (exp_avg, exp_avg_sq))
-        live = torch.zeros(size, dtype=torch.bool, device=self._device)
+        between = torch.ones(size, dtype=torch.bool, device=self._device)
         for first, n in zip(self._first, self._numel):
-            live[first * BLOCK:first * BLOCK + n] = True
+            between[first * BLOCK:first * BLOCK + n] = False
         for t in (m, v):
-            t.mul_(live)
+            t.masked_fill_(between, 0.0)          # (whatever lies between the parameters: NaN would not become 0 by a product)
         self._put_values(m, v)
         self._put_steps([int(step)] * len(self._list))
 
