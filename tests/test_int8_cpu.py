@@ -6,6 +6,7 @@ import torch
 
 from titanet_amd import _lib
 from titanet_amd.int8 import Int8Linear, Int8Rows, int8_matmul, quantize_rows
+from titanet_amd.metrics import cosine_scores
 
 
 def test_operands_must_live_on_a_device():
@@ -88,3 +89,16 @@ def test_products_of_operands_that_left_the_device():
                  lambda: layer(torch.ones(2, 3)), lambda: layer(torch.ones(64, 3, dtype=torch.bfloat16)), lambda: layer(torch.ones(0, 3))):
         with pytest.raises(RuntimeError, match="no CPU execution path"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+def test_cosine_scores_are_float32_whatever_the_embeddings_are(dtype):
+    """a row of zeros scores 0 against everything (in half precision the norm's lower bound of 1e-8 is no number of the type)"""
+    g = torch.Generator().manual_seed(1)
+    e, other = torch.randn(5, 24, generator=g).to(dtype), torch.randn(3, 24, generator=g).to(dtype)
+    e[2] = 0
+    for args in ((e,), (e, other)):
+        y = cosine_scores(*args)
+        a, b = (t.double() / t.double().norm(dim=1, keepdim=True).clamp(min=1e-8) for t in (args[0], args[-1]))
+        # both unit rows and a sum of 24 products, each rounded in float32
+        assert y.dtype == torch.float32 and float((y - a @ b.t()).abs().max()) <= 40 * 2.0 ** -24 and not y[2].any()

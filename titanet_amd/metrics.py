@@ -82,6 +82,7 @@ def cosine_scores(embeddings, enrolled=None, bits=32):
         raise ValueError(f"bits must be 8 or 32, got {bits!r}")
 
     def unit(e):
+        e = e.float()
         return e / e.norm(dim=1, keepdim=True).clamp(min=1e-8)       # F.cosine_similarity eps
     e = unit(embeddings)
     if bits == 32:
