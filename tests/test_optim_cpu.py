@@ -119,3 +119,14 @@ def test_hooks_of_a_state_dict_run_in_torchs_order():
         opt.load_state_dict(sd)
         assert sd["epoch"] == 4
     assert seen[0] == seen[1] and len(seen[0]) == 4
+
+
+@pytest.mark.parametrize("bad", [dict(amsgrad=True), dict(maximize=True), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0)])
+def test_a_refused_state_changes_nothing(bad):
+    opt = AdamW([{"params": [], "lr": 0.5}, {"params": []}])
+    state = opt.state_dict()
+    state["param_groups"][0]["lr"] = 0.25
+    state["param_groups"][1].update(bad)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(state)
+    assert [g["lr"] for g in opt.param_groups] == [0.5, 1e-3]

@@ -279,11 +279,14 @@ class AdamW(torch.optim.Optimizer):
             if e and (e["exp_avg"].numel() != n or e["exp_avg_sq"].numel() != n or (coded and (
                     e["exp_avg_scale"].numel() != (n + BLOCK - 1) // BLOCK or e["exp_avg_sq_scale"].numel() != (n + BLOCK - 1) // BLOCK))):
                 raise ValueError("loaded state dict has moments of another size")
-        for g, o in zip(groups, self.param_groups):
+        hypers = []
+        for g, o in zip(groups, self.param_groups):         # (everything is looked at before anything changes)
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("loaded state dict is of a variant (amsgrad, maximize) that AdamW does not have")
-            hyper = {k: v for k, v in g.items() if k in ("lr", "betas", "eps", "weight_decay")}
-            self._check_hyper({**o, **hyper})
+            hypers.append({k: v for k, v in g.items() if k in ("lr", "betas", "eps", "weight_decay")})
+            self._check_hyper({**o, **hypers[-1]})
+        steps = [int(float(e["step"])) if e else 0 for e in entries]
+        for g, o, hyper in zip(groups, self.param_groups, hypers):
             if "lr" in hyper and isinstance(o["lr"], torch.Tensor):
                 o["lr"].fill_(hyper.pop("lr"))               # (a captured step reads this tensor)
             elif isinstance(hyper.get("lr"), torch.Tensor):
@@ -295,9 +298,7 @@ class AdamW(torch.optim.Optimizer):
         m = torch.zeros(size, dtype=torch.int8 if coded else torch.float32, device=dev)
         v = torch.zeros(size, dtype=torch.uint8 if coded else torch.float32, device=dev)
         s1, s2 = torch.zeros(self.blocks, dtype=torch.float32, device=dev), torch.zeros(self.blocks, dtype=torch.float32, device=dev)
-        steps = []
         for e, first, n in zip(entries, self._first, self._numel):
-            steps.append(int(float(e["step"])) if e else 0)
             if not e:
                 continue
             lo, k = int(first) * BLOCK, int((n + BLOCK - 1) // BLOCK)
