@@ -698,3 +698,24 @@ def test_what_lies_between_loaded_moments_is_left_out(bits):
             opt.load_moments(m, v, step=1)
         for a, b in zip(opts[0].moments(), opts[1].moments()):
             assert torch.equal(a, b) and not b[~live].any()
+
+
+def test_parameters_taken_out_of_the_groups():
+    """moments belong to positions: what is left is stepped with its own, or the step is refused"""
+    ps = _tensors([300, 300, 300], torch.float32, 44)
+    for p, g in zip(ps, _grads([300, 300, 300], torch.float32, 45)):
+        p.grad = g
+    opt = AdamW([{"params": [p]} for p in ps])
+    opt.step()
+    kept = [p.clone() for p in ps]
+    last = opt.param_groups.pop()
+    opt.step()
+    assert not torch.equal(ps[0], kept[0]) and torch.equal(ps[2], kept[2]) and [int(e["step"]) for e in opt.state_dict()["state"].values()] == [2, 2]
+    kept = [p.clone() for p in ps]
+    first = opt.param_groups.pop(0)
+    with pytest.raises(RuntimeError, match="parameter list changed"):
+        opt.step()
+    assert all(torch.equal(p, k) for p, k in zip(ps, kept))
+    opt.param_groups[:] = [first] + opt.param_groups + [last]
+    opt.step()
+    assert [int(e["step"]) for e in opt.state_dict()["state"].values()] == [3, 3, 2]

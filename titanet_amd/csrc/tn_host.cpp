@@ -79,7 +79,7 @@ class Stepper {
   Stepper(int bits) : bits_(bits) {}
 
   void layout(std::vector<int64_t> numel, std::vector<int64_t> first, std::vector<int32_t> sets, int64_t blocks, at::Tensor exp_avg,
-              at::Tensor exp_avg_sq, std::optional<at::Tensor> scale1, std::optional<at::Tensor> scale2, at::Tensor steps, at::Tensor corr, at::Tensor owner) {
+              at::Tensor exp_avg_sq, std::optional<at::Tensor> scale1, std::optional<at::Tensor> scale2, at::Tensor steps, at::Tensor corr, at::Tensor owner, const py::list& params) {
     numel_ = std::move(numel);
     first_ = std::move(first);
     blocks_ = blocks;
@@ -90,6 +90,8 @@ class Stepper {
     steps_ = steps;
     corr_ = corr;
     owner_ = owner;
+    params_.clear();
+    for (const auto& p : params) params_.push_back(p.ptr());
     if (!norm_.defined()) norm_ = at::zeros({}, corr.options());
     put_sets(std::move(sets));
   }
@@ -124,6 +126,11 @@ class Stepper {
     std::vector<GroupWork> work;
     std::vector<char> active(numel_.size(), 0);
     work.reserve(groups.size());
+    // Moments belong to positions.  A parameter that was exchanged for another of its size keeps its position's; where some were taken out of
+    // the groups, those that are left must be at theirs.
+    size_t total = 0;
+    for (const auto& item : groups) total += py::reinterpret_borrow<py::list>(py::reinterpret_borrow<py::dict>(item)["params"]).size();
+    const bool whole = total == numel_.size();
     int32_t at = 0;
     for (const auto& item : groups) {
       const py::dict group = py::reinterpret_borrow<py::dict>(item);
@@ -134,7 +141,8 @@ class Stepper {
       for (Py_ssize_t k = 0; k < count; ++k) {
         PyObject* obj = PyList_GET_ITEM(params.ptr(), k);
         const int32_t i = at++;
-        TORCH_CHECK(THPVariable_Check(obj) && (size_t)i < numel_.size(), "AdamW: the parameter list changed; use add_param_group");
+        TORCH_CHECK(THPVariable_Check(obj) && (size_t)i < numel_.size() && (whole || obj == params_[i]),
+                    "AdamW: the parameter list changed; use add_param_group");
         const at::Tensor& p = THPVariable_Unpack(obj);
         const at::Tensor& given = p.grad();
         if (!given.defined()) continue;
@@ -276,6 +284,7 @@ class Stepper {
   int64_t blocks_ = 0;
   std::vector<int64_t> numel_, first_;
   std::vector<int32_t> sets_;
+  std::vector<PyObject*> params_;        // compared only: the Python side holds them
   bool captured_ = false;
   at::Tensor exp_avg_, exp_avg_sq_, scale1_, scale2_, steps_, corr_, owner_, norm_;
 };

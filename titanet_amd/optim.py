@@ -155,7 +155,7 @@ class AdamW(torch.optim.Optimizer):
         every = (self._numel + BLOCK - 1) // BLOCK
         self._owner = torch.from_numpy(np.repeat(np.arange(len(every), dtype=np.int32), every)).to(self._device)      # each block's parameter
         self._stepper.layout(self._numel.tolist(), self._first.tolist(), sets, self.blocks, self._exp_avg, self._exp_avg_sq, self._scale1,
-                             self._scale2, self._steps, self._corr, self._owner)
+                             self._scale2, self._steps, self._corr, self._owner, self._list)
 
     def _groups(self):
         """(group, index of its first parameter) in order"""
