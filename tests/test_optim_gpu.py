@@ -719,3 +719,39 @@ def test_parameters_taken_out_of_the_groups():
     opt.param_groups[:] = [first] + opt.param_groups + [last]
     opt.step()
     assert [int(e["step"]) for e in opt.state_dict()["state"].values()] == [3, 3, 2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_groups_are_two_optimizers(bits):
+    """no decay on the short tensors: a list of two groups gives the numbers of an optimizer for each"""
+    sizes, short = [70000, 256, 30001], [300, 17, 20000]
+    ps, qs = ([_tensors(s, torch.float32, 46 + k) for k, s in enumerate((sizes, short))] for _ in range(2))
+    opt = AdamW([{"params": ps[0], "weight_decay": 0.1}, {"params": ps[1], "weight_decay": 0.0, "betas": (0.8, 0.95)}], lr=1e-2, state_bits=bits)
+    apart = [AdamW(qs[0], lr=1e-2, weight_decay=0.1, state_bits=bits), AdamW(qs[1], lr=1e-2, weight_decay=0.0, betas=(0.8, 0.95), state_bits=bits)]
+    for k in range(3):
+        for group, twins, s in zip(ps, qs, (sizes, short)):
+            for p, q, g in zip(group, twins, _grads(s, torch.float32, 50 + k)):
+                p.grad = q.grad = g
+        opt.step()
+        for o in apart:
+            o.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps[0] + ps[1], qs[0] + qs[1])), k
+    for a, b, c in zip(opt.moments(), *(o.moments() for o in apart)):
+        assert torch.equal(a, torch.cat([b, c]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [None, 0.05, 1e9])
+def test_gradients_summed_over_ranks(clip, bits):
+    """two ranks' gradients added up and grad_mult = 1/2: the step of their mean, norm and clipping included"""
+    sizes = [5000, 33]
+    params = _tensors(sizes, torch.float32, 53)
+    opt = AdamW(params, lr=2e-3, weight_decay=0.1, state_bits=bits, max_grad_norm=clip, grad_mult=0.5)
+    oracles = [O.Tensor(_np(p), bits) for p in params]
+    for k in range(3):
+        a, b = _grads(sizes, torch.float32, 54 + k), _grads(sizes, torch.float32, 64 + k)
+        summed = [x + y for x, y in zip(a, b)]
+        norm = 0.5 * float(np.sqrt(sum((_np(g) ** 2).sum() for g in summed)))
+        _follow(opt, params, oracles, "fp32", bits, summed, lr=2e-3, wd=0.1, factor=0.5 * (O.clip_factor(norm, clip) if clip else 1.0))
+        if clip:
+            assert abs(float(opt.last_grad_norm) - norm) <= 2 * U * norm

@@ -213,7 +213,7 @@ class AdamW(torch.optim.Optimizer):
     def _put_steps(self, steps):
         """Sets every parameter's count.  Those of a group that are at one count are stepped together; once a step has been captured, only
         those that were so before: replays advance what they hold, and only these are known to stay at one count."""
-        old, first, sets = self._stepper.sets, {}, [0] * len(self._list)
+        old, first, sets = self._stepper.sets, {}, list(range(len(self._list)))
         for k, (group, at) in enumerate(self._groups()):
             for i in range(at, at + len(group["params"])):
                 sets[i] = first.setdefault((k, steps[i], old[i] if self._stepper.captured else None), i)
