@@ -755,3 +755,15 @@ def test_gradients_summed_over_ranks(clip, bits):
         _follow(opt, params, oracles, "fp32", bits, summed, lr=2e-3, wd=0.1, factor=0.5 * (O.clip_factor(norm, clip) if clip else 1.0))
         if clip:
             assert abs(float(opt.last_grad_norm) - norm) <= 2 * U * norm
+
+
+@pytest.mark.parametrize("sizes", [[700], [70001]])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping_by_factors_below_the_smallest_normal_float(bits, sizes):
+    params = _tensors(sizes, torch.float32, 3)
+    opt, oracles = AdamW(params, state_bits=bits, max_grad_norm=1e-9), [O.Tensor(_np(p), bits) for p in params]
+    for scale in (1e30, 1e32):
+        grads = [scale * g for g in _tensors(sizes, torch.float32, 4)]
+        norm = float(np.sqrt(sum((_np(g) ** 2).sum() for g in grads)))
+        assert O.clip_factor(norm, 1e-9) < 2.0 ** -130
+        _follow(opt, params, oracles, "fp32", bits, grads, lr=1e-3, factor=O.clip_factor(norm, 1e-9))

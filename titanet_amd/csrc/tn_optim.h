@@ -232,13 +232,20 @@ __device__ __forceinline__ void opt_step8_block(const OptStep& h, T* p, const fl
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void opt_step32(const OptStep& h, T* p, const float g[4], int64_t i, int64_t n, float* m, float* v) {
   const float b1 = (float)h.b1, b2 = (float)h.b2, w1 = (float)h.w1, w2 = (float)h.w2, factor = (float)h.factor;
-  float pv[4], mv[4], vv[4];
+  float pv[4], mv[4], vv[4], gf[4];
   opt_load4<WHOLE>(p, i, n, pv);
   opt_load4<WHOLE, true>(m, i, n, mv);              // (the padding of the last block is neither read nor written)
   opt_load4<WHOLE, true>(v, i, n, vv);
+  if (fabsf(factor) < 0x1p-126f) {                  // (uniform; a clipping factor that 32 bits cannot hold to their precision)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gf[j] = (float)((double)g[j] * h.factor);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gf[j] = g[j] * factor;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float gj = g[j] * factor;
+    const float gj = gf[j];
     mv[j] = b1 * mv[j] + w1 * gj;
     vv[j] = b2 * vv[j] + w2 * (gj * gj);
     pv[j] = pv[j] * h.decay - h.rate * opt_update(mv[j], vv[j], h.root, h.eps);
