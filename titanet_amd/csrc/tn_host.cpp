@@ -126,11 +126,7 @@ class Stepper {
     std::vector<GroupWork> work;
     std::vector<char> active(numel_.size(), 0);
     work.reserve(groups.size());
-    // Moments belong to positions.  A parameter that was exchanged for another of its size keeps its position's; where some were taken out of
-    // the groups, those that are left must be at theirs.
-    size_t total = 0;
-    for (const auto& item : groups) total += py::reinterpret_borrow<py::list>(py::reinterpret_borrow<py::dict>(item)["params"]).size();
-    const bool whole = total == numel_.size();
+    bool moved = false;
     int32_t at = 0;
     for (const auto& item : groups) {
       const py::dict group = py::reinterpret_borrow<py::dict>(item);
@@ -141,8 +137,8 @@ class Stepper {
       for (Py_ssize_t k = 0; k < count; ++k) {
         PyObject* obj = PyList_GET_ITEM(params.ptr(), k);
         const int32_t i = at++;
-        TORCH_CHECK(THPVariable_Check(obj) && (size_t)i < numel_.size() && (whole || obj == params_[i]),
-                    "AdamW: the parameter list changed; use add_param_group");
+        TORCH_CHECK(THPVariable_Check(obj) && (size_t)i < numel_.size(), "AdamW: the parameter list changed; use add_param_group");
+        moved |= obj != params_[i];
         const at::Tensor& p = THPVariable_Unpack(obj);
         const at::Tensor& given = p.grad();
         if (!given.defined()) continue;
@@ -173,6 +169,9 @@ class Stepper {
       hyper(group, dev, capturing, w);
       work.push_back(std::move(w));
     }
+    // Moments belong to positions.  A parameter that was exchanged for another of its size keeps its position's; where some were taken out of
+    // the groups, those that are left must be at theirs.
+    TORCH_CHECK(!moved || (size_t)at == numel_.size(), "AdamW: the parameter list changed; use add_param_group");
     if (work.empty()) return std::nullopt;
     split(active, capturing);
     // Every tensor has a count of its own, at its own place on the device, which is advanced in every step that it takes part in.  Tensors of
