@@ -165,7 +165,9 @@ __device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) {
 // made by every workgroup for itself in LDS while the first weight loads are on their way, so one launch does it all.  NW waves
 // share a tile of 32 channels by splitting K in KS parts (joined through LDS: integer sums, any order gives the same) or work on
 // NW / KS tiles.  Bound by the latency of load - maximum - codes - product for small weights (1 x 7205 x 192 4.6 us, 16 x 192 x 1536 from
-// float 6.3 us; quantised by a launch of its own and multiplied in tiles they took 8.4 and 28), by HBM for large ones.
+// float 6.3 us; quantised by a launch of its own and multiplied in tiles they took 8.4 and 28), by HBM for one row
+// against a large one (1 x 100003 x 1536 34 us, 4.5 TB/s).  More rows make their codes anew in each of up to 2048 workgroups: 16 rows
+// 43 us, 32 rows 75 (2.2 TB/s).
 struct FewArgs {
   const void* x;                      // rows of X, or codes with scales sa
   Int8Args g;
@@ -341,11 +343,12 @@ struct Q8Pair {
 // row / 4 & 3 (64), applied to the source address of the LDS-DMA and undone by the fragment reads: sixteen rows of one chunk fall into
 // sixteen different groups of the 64 banks.  Weight row 2 i + j of a wave's 64-column block lies at image row 32 j + i: a lane then owns
 // two neighbouring columns and stores them together.
-// Bound by stores for short sums (4708 x 50021 x 192 to float32: 226 us, 4.2 TB/s) and for long ones by the matrix pipe at the clock
-// that the chip's power leaves it: 2.9 POP/s fed from registers alone; 76800 x 1536 x 1536 in 290 us, where the library's product to
-// 32-bit integers takes 268, 76800 x 1024 x 1024 in 132 (148), 76800 x 512 x 512 in 41 - 48 (56), 2048 x 2048 x 2048 in 17 (21).  Built and
-// not kept: tiles of 256 x 256 by 8 waves, persistent with LDS-DMA (267 us) or one to a workgroup through registers, one or two steps
-// ahead (272 - 308, 288), 128 x 256 and 256 x 128 by 4 waves (278 - 297): within a tenth on the largest shape, behind on the others.
+// Bound by stores for short sums (4708 x 50021 x 192 to float32: 221 us, 4.3 TB/s) and for long ones by the loop, which waits at two
+// workgroup barriers and for its LDS reads in every step: at 76800 x 1536 x 1536 (241 - 290 us, 1.4 POP/s) the matrix pipe is busy in 36 %
+// of the cycles, at a clock of 1.86 GHz; fed from registers alone it reaches 2.9 POP/s.  The library's product to 32-bit integers takes
+// 268 us there; 76800 x 1024 x 1024 132 (library 148), 76800 x 512 x 512 41 - 48 (56), 2048 x 2048 x 2048 17 (21).  Built and not kept:
+// tiles of 256 x 256 by 8 waves, persistent with LDS-DMA (267 us) or one to a workgroup through registers, one or two steps ahead
+// (272 - 308, 288), 128 x 256 and 256 x 128 by 4 waves (278 - 297): within a tenth on the largest shape, behind on the others.
 template <typename Y, int TM, int TN, int STEP, int NS>
 __global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles_m, int tiles_n, bool down) {
   constexpr int STAGE = (TM + TN) * STEP, CPR = STEP / 16, RP = 64 / CPR, SH = STEP == 128 ? 1 : 2;

@@ -13,7 +13,7 @@
 
 namespace {
 
-// Elements of one workgroup of the step, 32- and 8-bit moments.  Timed at 1024 / 2048 / 4096 / 8192: 24.7 M elements fp32 and 32 bits
+// Elements of one workgroup of the step, 32- and 8-bit moments.  Timed at 1024 / 2048 / 4096 / 8192: 26.1 M elements fp32 and 32 bits
 // 144.1 / 144.4 / 146.9 / 150.6 us, 6.2 M with their norm 45 / 42.2 / 44.5 / 46; 64 M elements and 8 bits 299 / 309 / 312 / 317 us.
 constexpr int OPT_CHUNK32 = 2048, OPT_CHUNK8 = 1024;
 constexpr int SUM_CHUNK = 8192;        // elements behind one partial sum of the norm
@@ -28,9 +28,10 @@ struct SumList {
   uint32_t end[OPT_LIST];              // chunks of this launch before the end of tensor i (ascending)
 };
 
-// One partial sum of squares per chunk of SUM_CHUNK elements, in 64 bits (no gradient of a 32-bit type overflows there, and the
-// order of the sum is fixed: two runs give the same norm).  Bound by memory: all of a chunk's loads are asked for at once (6.2 M float
-// gradients 7.2 us, 3.5 TB/s; with a loop over chunks twice as long 13 us).
+// One partial sum of squares per chunk of SUM_CHUNK elements, in 64 bits (no gradient of a 32-bit type overflows there).  The order of
+// the sum is fixed: two runs over the same tensors give the same norm.  Tensors that lie next to each other are summed as one run, so
+// another layout can end its chunks elsewhere and differ in the last places of 64 bits.  Bound by memory: all of a chunk's loads are
+// asked for at once (6.2 M float gradients 7.2 us, 3.5 TB/s; with a loop over chunks twice as long 13 us).
 template <typename T>
 __global__ __launch_bounds__(256) void grad_sumsq_kernel(SumList list, double* __restrict__ partials) {
   const int t = opt_find(list.end, OPT_LIST, blockIdx.x);
@@ -170,8 +171,8 @@ __device__ __forceinline__ OptStep opt_step_of(const OptHyper& h, const float4& 
   return {h.b1, h.b2, h.w1, h.w2, factor, c.x, c.y, c.z, h.eps};
 }
 
-// 32-bit moments: four elements to a lane, 28 bytes of an element (float parameters) moved once.  Bound by HBM: 24.7 M elements in
-// 130 us, 5.3 TB/s, where a large copy reaches 4.8; moments and gradients go past the caches (142 us with them left there).
+// 32-bit moments: four elements to a lane, 28 bytes of an element (float parameters) moved once.  Bound by HBM: 26.1 M elements in
+// 130 us, 5.6 TB/s, where a large copy reaches 4.8; moments and gradients go past the caches (142 us with them left there).
 // EACH: a run's tensors may be at different counts, every block of 256 elements (a wave's four times 64) has the numbers of its own.
 template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, float* __restrict__ exp_avg, float* __restrict__ exp_avg_sq,
@@ -214,8 +215,8 @@ __global__ __launch_bounds__(256) void adamw32_kernel(OptList list, OptHyper h, 
 
 // 8-bit moments: one wave holds one block of 256 elements, four to a lane, so that the block's maxima are a reduction over the
 // wave and neither LDS nor a barrier is needed.  16 bytes of an element (float parameters): 64 M elements in 187 us, 5.5 TB/s.  With
-// 16-bit parameters (10 bytes) the vector pipe bounds it: some 450 instructions a block, a fifth of them in 64 bits (7.9 M bfloat16
-// elements in 26 us, 3.1 TB/s; 37 us with integer squares, 64-bit quotients and a shuffled maximum).
+// 16-bit parameters (10 bytes) the vector pipe bounds it: some 450 instructions a block, a fifth of them in the 64 bits that
+// decide every code (7.9 M bfloat16 elements in 26 us, 3.1 TB/s; 37 us with integer squares, 64-bit quotients and a shuffled maximum).
 template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw8_kernel(OptList list, OptHyper h, int8_t* __restrict__ exp_avg, uint8_t* __restrict__ exp_avg_sq,
                                                      float* __restrict__ scale1, float* __restrict__ scale2,

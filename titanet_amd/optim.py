@@ -26,9 +26,9 @@ def _dev(tensor):
 
 
 def grad_norm(tensors):
-    """The 2-norm of all elements of ``tensors`` together, as a 0-dim float32 tensor on their device.  Summed in 64 bits in a
-    fixed order: two calls on the same values give the same number.  float32, bfloat16 and float16 may be mixed.  The number is for
-    reading: it takes no part in autograd."""
+    """The 2-norm of all elements of ``tensors`` together, as a 0-dim float32 tensor on their device.  Summed in 64 bits in an
+    order that goes by the tensors and by which of them lie next to each other in memory: two calls on the same tensors give the same
+    number.  float32, bfloat16 and float16 may be mixed.  The number is for reading: it takes no part in autograd."""
     return _lib.load_host().grad_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors))
 
 
@@ -50,8 +50,8 @@ class AdamW(torch.optim.Optimizer):
     ``grad_mult`` multiplies the gradients before everything else (1 / world size behind a summing all-reduce).
 
     ``lr`` may be a 0-dim float32 tensor on the device; a step can be captured into a graph only then (a number would be frozen
-    into the graph).  The graph then reads and writes the optimizer's buffers: keep the optimizer as long as the graph.  No
-    parameter group can be added any more; loading a state and eager steps of all or some parameters go on as before.
+    into the graph, as the other hyper-parameters are).  The graph then reads and writes the optimizer's buffers: keep the optimizer as
+    long as the graph.  No parameter group can be added any more; loading a state and eager steps of all or some parameters go on.
 
     Parameters whose ``.grad`` is None are left alone and keep a step count of their own."""
 
