@@ -767,3 +767,30 @@ def test_clipping_by_factors_below_the_smallest_normal_float(bits, sizes):
         norm = float(np.sqrt(sum((_np(g) ** 2).sum() for g in grads)))
         assert O.clip_factor(norm, 1e-9) < 2.0 ** -130
         _follow(opt, params, oracles, "fp32", bits, grads, lr=1e-3, factor=O.clip_factor(norm, 1e-9))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [None, 1e9])
+def test_more_tensors_than_one_launch_counts(clip, bits):
+    """1300 tensors, empty ones among them, against optimizers of a quarter each; then a step of some and a captured one"""
+    sizes = [(37 * i) % 300 for i in range(1300)]
+    ps, qs = _tensors(sizes, torch.float32, 70), _tensors(sizes, torch.float32, 70)
+    kw = dict(weight_decay=0.1, state_bits=bits, max_grad_norm=clip)
+    opt = AdamW(ps, lr=torch.full((), 1e-2, device="cuda"), **kw)
+    apart = [AdamW(qs[lo:lo + 325], lr=torch.full((), 1e-2, device="cuda"), **kw) for lo in range(0, 1300, 325)]
+    graph = torch.cuda.CUDAGraph()
+    held = _grads(sizes, torch.float32, 71)
+    for k in range(6):
+        captured = k >= 4
+        for i, (p, q, g) in enumerate(zip(ps, qs, held if captured else _grads(sizes, torch.float32, 72 + k))):
+            p.grad = q.grad = None if k == 2 and i % 3 == 0 else g
+        if k == 4:
+            with torch.cuda.graph(graph):
+                opt.step()
+        graph.replay() if captured else opt.step()
+        for o in apart:
+            o.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
+    steps = [int(e["step"]) for e in opt.state_dict()["state"].values()]
+    assert steps == [int(e["step"]) for o in apart for e in o.state_dict()["state"].values()] and set(steps) == {5, 6}
