@@ -306,3 +306,17 @@ def test_a_product_is_not_traced():
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, x, check_trace=False)
     assert layer(x).shape == (3, 4)
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_scales_of_either_sign_and_any_size(m):
+    """codes and scales in hand: the sum times one of them may leave float32, the product does not"""
+    g = torch.Generator().manual_seed(34)
+    a, b = (torch.randint(-127, 128, (r, 96), generator=g, dtype=torch.int8).cuda() for r in (m, 21))
+    sa, sb = torch.full((m,), -2.0 ** 120, device="cuda"), torch.full((21,), 2.0 ** -30, device="cuda")
+    sa[1::2], sb[::3] = 2.0 ** -140, -2.0 ** -20
+    y = int8_matmul(Int8Rows(a, sa), Int8Rows(b, sb))
+    want, part = O.product(a.cpu().numpy().astype(np.int64), _np(sa), b.cpu().numpy().astype(np.int64), _np(sb))
+    _compare(y, want, part, "fp32")
+    y = int8_matmul(Int8Rows(b, sb), Int8Rows(a, sa))
+    _compare(y, want.T, part.T, "fp32")

@@ -156,7 +156,7 @@ constexpr float Q8_FAR = 0x1p96f;
 template <typename T, bool FAR>
 __device__ __forceinline__ T q8_out(int acc, float sa, float sb, float bias) {
   if constexpr (!FAR) return (T)((float)acc * sa * sb + bias);
-  const bool last = sa >= Q8_FAR;
+  const bool last = fabsf(sa) >= Q8_FAR;
   return (T)((float)acc * (last ? sb : sa) * (last ? sa : sb) + bias);
 }
 
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Args g, int tiles
   float* sc = reinterpret_cast<float*>(smem);       // [TM] token scales, [TN] channel scales, [TN] bias, a wave's word each: a far token scale
   static_assert(TM <= 128 && (TM + 2 * TN + 2) * 4 <= STAGE, "token scales come from the first two waves");
   if (threadIdx.x < TM) sc[threadIdx.x] = in_sa;
-  if (threadIdx.x < 128) sc[TM + 2 * TN + wave] = __ballot(in_sa >= Q8_FAR) ? 1.f : 0.f;
+  if (threadIdx.x < 128) sc[TM + 2 * TN + wave] = __ballot(fabsf(in_sa) >= Q8_FAR) ? 1.f : 0.f;
   if (threadIdx.x < TN) {
     sc[TM + threadIdx.x] = in_sb;
     sc[TM + TN + threadIdx.x] = in_bias;
