@@ -130,3 +130,17 @@ def test_a_refused_state_changes_nothing(bad):
     with pytest.raises(ValueError):
         opt.load_state_dict(state)
     assert [g["lr"] for g in opt.param_groups] == [0.5, 1e-3]
+
+
+@pytest.mark.parametrize("bad", [0.0, -1.0, float("nan")])
+def test_a_norm_assigned_later_is_checked(bad):
+    opt = AdamW([{"params": []}], max_grad_norm=1.0)
+    opt.step()
+    opt.max_grad_norm = bad
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        opt.step()
+    opt.max_grad_norm = None
+    opt.step()
+    for mult in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="grad_mult"):
+            AdamW([{"params": []}], grad_mult=mult)

@@ -10,6 +10,7 @@ the clipping factor and a learning rate given as a device tensor are read on the
 replayed, and a step whose gradient norm is not finite leaves everything as it was.  There is no CPU fallback.
 """
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -58,8 +59,9 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, grad_mult=1.0):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
-        if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
-            raise ValueError(f"max_grad_norm must be above 0 or None, got {max_grad_norm!r}")
+        self._check_norm(max_grad_norm)
+        if not math.isfinite(grad_mult):
+            raise ValueError(f"grad_mult must be a finite number, got {grad_mult!r}")
         self.state_bits, self.max_grad_norm, self.grad_mult = state_bits, max_grad_norm, float(grad_mult)
         self.last_grad_norm = None
         self._native = _lib.load()
@@ -110,6 +112,11 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         self._device = device
         self._extend(new)
+
+    @staticmethod
+    def _check_norm(max_grad_norm):
+        if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
+            raise ValueError(f"max_grad_norm must be above 0 or None, got {max_grad_norm!r}")
 
     @staticmethod
     def _check_hyper(g):
@@ -167,6 +174,7 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ the step
     def step(self, closure=None):
         loss = None
+        self._check_norm(self.max_grad_norm)          # (it may have been assigned)
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
