@@ -6,7 +6,7 @@ import torch
 
 from titanet_amd import _lib
 from titanet_amd.int8 import Int8Linear, Int8Rows, int8_matmul, quantize_rows
-from titanet_amd.metrics import cosine_scores
+from titanet_amd.metrics import cosine_scores, verification_test
 
 
 def test_operands_must_live_on_a_device():
@@ -102,3 +102,11 @@ def test_cosine_scores_are_float32_whatever_the_embeddings_are(dtype):
         a, b = (t.double() / t.double().norm(dim=1, keepdim=True).clamp(min=1e-8) for t in (args[0], args[-1]))
         # both unit rows and a sum of 24 products, each rounded in float32
         assert y.dtype == torch.float32 and float((y - a @ b.t()).abs().max()) <= 40 * 2.0 ** -24 and not y[2].any()
+
+
+def test_scores_refuse_before_they_compute():
+    rows = Int8Rows._of(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4), 3)
+    with pytest.raises(TypeError, match="bits=8"):
+        cosine_scores(torch.ones(2, 3), rows)
+    with pytest.raises(ValueError, match="score_bits"):
+        verification_test(None, [], [], score_bits=16)

@@ -84,10 +84,12 @@ def cosine_scores(embeddings, enrolled=None, bits=32):
     def unit(e):
         e = e.float()
         return e / e.norm(dim=1, keepdim=True).clamp(min=1e-8)       # F.cosine_similarity eps
+    from .int8 import Int8Rows, int8_matmul, quantize_rows
+    if bits == 32 and isinstance(enrolled, Int8Rows):
+        raise TypeError("enrolled Int8Rows are scored with bits=8")
     e = unit(embeddings)
     if bits == 32:
         return e @ (e if enrolled is None else unit(enrolled)).t()
-    from .int8 import Int8Rows, int8_matmul, quantize_rows
     rows = quantize_rows(e) if enrolled is None else enrolled if isinstance(enrolled, Int8Rows) else quantize_rows(unit(enrolled))
     return int8_matmul(rows if enrolled is None else e, rows, out_dtype=torch.float32)
 
@@ -102,6 +104,8 @@ def verification_test(model, spectrograms, speakers, mindcf_p_target=1e-2, mindc
     with the cosine similarity of the L2-normalised embeddings.
     ``score_bits=8``: the pairs are scored in 8-bit integers (:func:`cosine_scores`).
     spectrograms: list of [n_mels, T_i] or [1, n_mels, T_i] tensors; speakers: list of ids."""
+    if score_bits not in (8, 32):
+        raise ValueError(f"score_bits must be 8 or 32, got {score_bits!r}")
     was_training = model.training
     model.eval()
     dev = model.flat_parameters().device
